@@ -1,0 +1,114 @@
+#include "branch.hpp"
+
+#include <cmath>
+
+#include "kernels.hpp"
+
+namespace celeg {
+
+namespace {
+void need(bool ok, const char* message) {
+    if (!ok) throw ArgumentError(message);
+}
+void floats(DType dtype, const char* message) { need(dtype == DType::F32 || dtype == DType::BF16, message); }
+
+// the pages and the table of a group, as the kernels address them
+void check_cache(const KVView& kv) {
+    floats(kv.dtype, "cache: the pages are float32 or bfloat16");
+    need(kv.k && kv.table, "cache: the pages or the table are missing");
+    need(kv.n_pages > 0 && kv.n_layers > 0 && kv.kv_heads > 0 && kv.page_tokens > 0 && kv.head_dim > 0 && kv.v_head_dim >= 0 &&
+             kv.table_rows > 0 && kv.table_stride > 0, "cache: sizes must be positive");
+    need((kv.v_head_dim > 0) == (kv.v != nullptr), "cache: values and their width come together (keys only: neither)");
+    need(static_cast<long long>(kv.table_stride) * kv.page_tokens < (1LL << 31) - 4096, "cache: a request's places must fit 31 bits");
+    need(static_cast<long long>(kv.n_layers) * kv.kv_heads <= 65535, "cache: more than 65,535 layers times heads");
+}
+}  // namespace
+
+// ---------------------------------------------------------------------------- log probabilities
+static void check(const TokenLogprobs& a) {
+    floats(a.dtype, "token_logprobs: logits must be float32 or bfloat16");
+    need(a.rows >= 0 && a.rows < (1LL << 31), "token_logprobs: the number of rows must be in [0, 2^31)");
+    need(a.vocab > 0 && a.vocab <= (1LL << 24), "token_logprobs: the vocabulary must be in [1, 2^24]");
+    need(a.per_row >= 0 && a.per_row <= TokenLogprobs::MAX_PER_ROW, "token_logprobs: up to 8 tokens a row");
+    need(a.top >= 0 && a.top <= TokenLogprobs::MAX_TOP && a.top <= a.vocab, "token_logprobs: top must be in [0, 128] and not above the vocabulary");
+    need(a.row_stride >= 0 && (a.rows <= 1 || a.row_stride == 0 || a.row_stride >= a.vocab),
+         "token_logprobs: rows must not overlap in part (a row stride of 0 or at least the vocabulary)");
+    if (a.rows == 0) return;
+    need(a.logits != nullptr, "token_logprobs: the logits are missing");
+    need(a.per_row == 0 || (a.tokens && a.logprobs && a.ranks), "token_logprobs: tokens, logprobs and ranks come together");
+    need(a.top == 0 || (a.top_ids && a.top_logprobs), "token_logprobs: top_ids and top_logprobs are missing");
+}
+
+size_t token_logprobs_workspace(const TokenLogprobs& a) {
+    (void)a;
+    return 0;
+}
+
+void token_logprobs(const TokenLogprobs& a, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    check(a);
+    (void)workspace;
+    (void)workspace_bytes;
+    if (a.rows == 0) return;
+    kernel_check(celeg_logprobs_rows(a.logits, static_cast<int>(a.dtype), a.rows, static_cast<int>(a.vocab), a.row_stride, a.tokens,
+                                     a.per_row, a.top, a.logprobs, a.ranks, a.entropy, a.top_ids, a.top_logprobs, stream),
+                 "token_logprobs");
+}
+
+// ---------------------------------------------------------------------------- attention of trees
+static void check(const TreeAttention& a, const KVView& kv) {
+    check_cache(kv);
+    need(kv.v_head_dim == kv.head_dim, "tree_attention: values of the keys' width only");
+    need(kv.layer >= 0 && kv.layer < kv.n_layers, "tree_attention: layer outside the cache");
+    need(kv.head_dim <= TreeAttention::MAX_HEAD_DIM, "tree_attention: heads of up to 256");
+    need(a.rows >= 0 && a.requests >= 0, "tree_attention: negative counts");
+    need(a.heads > 0 && a.heads <= 65535 && a.heads % kv.kv_heads == 0, "tree_attention: heads must be a multiple of the cache's key/value heads");
+    need(a.max_nodes > 0 && a.max_nodes <= TreeAttention::MAX_NODES, "tree_attention: max_nodes must be in [1, 256]");
+    need(static_cast<long long>(a.requests) * a.max_nodes <= 65535, "tree_attention: more than 65,535 requests times max_nodes");
+    need(a.window >= 0 && a.max_context >= 0, "tree_attention: window and max_context must not be negative");
+    need(std::isfinite(a.scale), "tree_attention: the scale must be finite");
+    const long long width = static_cast<long long>(a.heads) * kv.head_dim;
+    need(a.rows <= 1 || a.q_stride >= width, "tree_attention: the rows of q overlap");
+    need(a.q_stride >= 0 && a.q_stride < (1LL << 31), "tree_attention: the row stride of q must be in [0, 2^31)");
+    if (a.rows == 0 || a.requests == 0) return;
+    need(a.q && a.out && a.slots && a.starts && a.offsets && a.parents, "tree_attention: an argument is missing");
+}
+
+size_t tree_attention_workspace(const TreeAttention& a, const KVView& kv) {
+    (void)a;
+    (void)kv;
+    return 0;
+}
+
+void tree_attention(const TreeAttention& a, const KVView& kv, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    check(a, kv);
+    (void)workspace;
+    (void)workspace_bytes;
+    if (a.rows == 0 || a.requests == 0) return;
+    kernel_check(celeg_tree_attention_general(a.q, static_cast<int>(a.q_stride), static_cast<int>(kv.dtype), kv.k, kv.v, kv.n_pages,
+                                              kv.n_layers, kv.layer, a.heads, kv.kv_heads, kv.head_dim, kv.page_tokens, kv.table,
+                                              kv.table_rows, kv.table_stride, a.slots, a.starts, a.offsets, a.parents, a.requests, a.rows,
+                                              a.max_nodes, a.scale, a.window, a.out, stream), "tree_attention");
+}
+
+// ---------------------------------------------------------------------------- tokens and pages
+void move_tokens(const MoveTokens& a, const KVView& kv, hipStream_t stream) {
+    check_cache(kv);
+    need(a.requests >= 0 && a.n_places >= 0, "move_tokens: negative counts");
+    if (a.requests == 0 || a.n_places == 0) return;
+    need(a.src_slots && a.dst_slots && a.offsets && a.places && a.dst_starts, "move_tokens: an argument is missing");
+    kernel_check(celeg_move_token_list(kv.k, kv.v, static_cast<int>(kv.dtype), kv.n_pages, kv.n_layers, kv.kv_heads, kv.page_tokens,
+                                       kv.head_dim, kv.v_head_dim, kv.table, kv.table_rows, kv.table_stride, a.src_slots, a.dst_slots,
+                                       a.offsets, a.places, a.dst_starts, a.requests, a.n_places, stream), "move_tokens");
+}
+
+void copy_pages(const KVView& kv, const int* src, const int* dst, int n, hipStream_t stream) {
+    check_cache(kv);
+    need(n >= 0, "copy_pages: a negative count");
+    if (n == 0) return;
+    need(src && dst, "copy_pages: the lists of pages are missing");
+    const size_t per_dim = static_cast<size_t>(kv.n_layers) * kv.kv_heads * kv.page_tokens * dtype_size(kv.dtype);
+    kernel_check(celeg_copy_page_list(kv.k, kv.v, per_dim * kv.head_dim, per_dim * kv.v_head_dim, kv.n_pages, src, dst, n, stream),
+                 "copy_pages");
+}
+
+}  // namespace celeg

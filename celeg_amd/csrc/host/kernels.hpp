@@ -266,4 +266,18 @@ int celeg_gla_prepare(const void* q, int ldq, const void* k, int ldk, const void
 int celeg_channel_scan(const float* qk, const float* v, const float* decay, const float* beta, int ld_beta, float* state,
                        size_t state_stride, const int* cu_seqlens, const int* seq_slot, float* out, int n_seqs, int G, int H, int D,
                        int V, int general, hipStream_t stream);
+// token_logprobs.hip
+int celeg_logprobs_rows(const void* logits, int dtype, long long rows, int vocab, long long row_stride, const int* tokens, int per_row,
+                        int top, float* logprobs, int* ranks, float* entropy, int* top_ids, float* top_logprobs, hipStream_t stream);
+// tree_attention.hip
+int celeg_tree_attention_general(const void* q, int ldq, int dtype, const void* k_pool, const void* v_pool, int n_pages, int n_layers,
+                                 int layer, int heads, int kv_heads, int head_dim, int page_tokens, const int* table, int table_rows,
+                                 int table_stride, const int* slots, const int* starts, const int* offsets, const int* parents,
+                                 int n_requests, int n_rows, int max_nodes, float scale, int window, void* out, hipStream_t stream);
+// cache_copy.hip
+int celeg_copy_page_list(void* k, void* v, size_t k_bytes, size_t v_bytes, int n_pages, const int* src, const int* dst, int n,
+                         hipStream_t stream);
+int celeg_move_token_list(void* k, void* v, int dtype, int n_pages, int n_layers, int kv_heads, int page_tokens, int head_dim,
+                          int v_head_dim, const int* table, int table_rows, int table_stride, const int* src_slots, const int* dst_slots,
+                          const int* offsets, const int* places, const int* dst_starts, int n, int n_places, hipStream_t stream);
 }

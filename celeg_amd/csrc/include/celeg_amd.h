@@ -226,6 +226,79 @@ const char* celeg_ops_call(celeg_ops* ops, const char* op, const char* args_json
  * Needs no GPU. */
 const char* celeg_reference_call(const char* op, const char* args_json);
 
+/* ---- operators for requests that go on in several ways ----
+ * What a program calls between a model's steps: log probabilities of given tokens, attention of a tree of drafted
+ * tokens over a paged cache, the tokens of a kept path brought together, pages copied.  Each call launches on `stream`
+ * (a hipStream_t of the current device, which all addresses belong to) and keeps nothing: no handle, no state; calls from
+ * several threads, on several streams, or recorded into graphs, are independent as far as their memory is.  Wrong
+ * arguments are refused with CELEG_INVALID_ARGUMENT before anything is launched (without a GPU too).  Structs carry their size
+ * in struct_size.  dtype: 0 float32, 1 bfloat16.  A call with nothing to do (no rows, no requests, no pages) is CELEG_OK.
+ * Workspaces: 16-byte aligned device memory of the size that the *_workspace function gives for the same arguments (it does not
+ * look at addresses of data); they hold nothing between calls, and two calls that may run at the same time need one each. */
+
+/* All layers of one group of pages: k [n_pages, n_layers, kv_heads, page_tokens, head_dim], v [n_pages, n_layers, kv_heads,
+ * v_head_dim, page_tokens] (null with v_head_dim 0: keys only), table [table_rows, table_stride]: row s names the pages of slot s.
+ * An entry that is no page of the pool names nothing: keys there are not seen, nothing is read or written. */
+typedef struct celeg_paged_cache {
+    size_t struct_size;
+    void *k, *v;
+    const int32_t* table;
+    int32_t dtype, n_pages, n_layers, kv_heads, page_tokens, head_dim, v_head_dim, table_rows, table_stride;
+} celeg_paged_cache;
+
+/* For every row of logits [rows, vocab] (row_stride elements apart): of up to 8 tokens a row their log probabilities and ranks
+ * (how many logits stand ahead: larger ones, and equal ones of lower index), the entropy (nats; null: not wanted), and the
+ * `top` (up to 128) best tokens by logit, equal ones by index, with their log probabilities.  Sums are 32-bit.
+ * A token outside [0, vocab): NaN and rank -1.  A row that is no distribution (a NaN, a +inf, nothing but -inf): NaN for
+ * log probabilities and entropy; with a NaN in it also ranks and ids of -1. */
+typedef struct celeg_token_logprobs_args {
+    size_t struct_size;
+    const void* logits;
+    int64_t rows, vocab, row_stride;
+    int32_t dtype, per_row, top;
+    const int32_t* tokens;       /* [rows, per_row] */
+    float* logprobs;             /* [rows, per_row] */
+    int32_t* ranks;              /* [rows, per_row] */
+    float* entropy;              /* [rows] */
+    int32_t* top_ids;            /* [rows, top] */
+    float* top_logprobs;         /* [rows, top] */
+} celeg_token_logprobs_args;
+celeg_status celeg_token_logprobs_workspace(const celeg_token_logprobs_args* args, size_t* bytes);
+celeg_status celeg_token_logprobs(const celeg_token_logprobs_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention of drafted trees.  Request r has rows offsets[r] .. offsets[r + 1] - 1 of q and out (up to max_nodes, at most
+ * 256): the nodes of its tree, whose keys and values lie behind its context of starts[r] tokens, node i's at place starts[r] + i
+ * of slot slots[r].  parents[row] is the index inside the tree of the node's parent, lower than its own (anything else: a
+ * root).  A node sees the context, its ancestors and itself, with a window only what stands fewer than `window` positions
+ * before its own, starts[r] + depth.  out = softmax(scale q . k) v [rows, heads * head_dim], in the pages' dtype like q (rows
+ * q_stride elements apart).  Rows of no request, of a request behind max_nodes, or of a slot outside the table are left as
+ * they were.  What a node does not see may hold anything, infinities and NaN included. */
+typedef struct celeg_tree_attention_args {
+    size_t struct_size;
+    const void* q;
+    int64_t q_stride;
+    void* out;
+    int32_t rows, heads, requests, layer;
+    const int32_t *slots, *starts, *offsets, *parents;
+    float scale;
+    int32_t window, max_nodes;
+    int32_t max_context;         /* about the longest context, 0: what the table holds; only the cut of the work hangs on it */
+} celeg_tree_attention_args;
+celeg_status celeg_tree_attention_workspace(const celeg_tree_attention_args* args, const celeg_paged_cache* cache, size_t* bytes);
+celeg_status celeg_tree_attention(const celeg_tree_attention_args* args, const celeg_paged_cache* cache, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
+/* Keys and values of all layers moved: entry i of request r (entries offsets[r] .. offsets[r + 1] - 1 of places) goes from place
+ * places[entry] of slot src_slots[r] to place dst_starts[r] + i of slot dst_slots[r].  Within one slot the places have to rise,
+ * none above where its token goes to (place >= dst_starts[r] + i); between two slots any order will do.  No place that one request writes
+ * may be one that another reads or writes.  A place outside the table, or on no page, is left out. */
+celeg_status celeg_move_tokens(const celeg_paged_cache* cache, int32_t requests, const int32_t* src_slots, const int32_t* dst_slots,
+                               const int32_t* offsets, const int32_t* places, int32_t n_places, const int32_t* dst_starts, void* stream);
+
+/* Pages src[i] copied to dst[i], all layers; a page may be copied from several times, but written once and not read as well.  Pairs
+ * that name no page of the pool are left out. */
+celeg_status celeg_copy_pages(const celeg_paged_cache* cache, const int32_t* src, const int32_t* dst, int32_t n, void* stream);
+
 /* ---- without a GPU: what a folder holds ---- */
 /* JSON {"config", "spec", "expected_tensors": [{"name", "shape", "kind", "init", "also"}]} of a model
  * folder (config.json, generation_config.json, and the checkpoint's tensor names for what they leave out) */

@@ -83,6 +83,25 @@ class ForwardArgs(ctypes.Structure):
                 ("dtype", c_int32)]
 
 
+class PagedCacheStruct(ctypes.Structure):
+    _fields_ = [("struct_size", c_size_t), ("k", c_void_p), ("v", c_void_p), ("table", c_void_p)] + \
+               [(name, c_int32) for name in ("dtype", "n_pages", "n_layers", "kv_heads", "page_tokens", "head_dim", "v_head_dim",
+                                             "table_rows", "table_stride")]
+
+
+class TokenLogprobsArgs(ctypes.Structure):
+    _fields_ = [("struct_size", c_size_t), ("logits", c_void_p), ("rows", c_int64), ("vocab", c_int64), ("row_stride", c_int64),
+                ("dtype", c_int32), ("per_row", c_int32), ("top", c_int32)] + \
+               [(name, c_void_p) for name in ("tokens", "logprobs", "ranks", "entropy", "top_ids", "top_logprobs")]
+
+
+class TreeAttentionArgs(ctypes.Structure):
+    _fields_ = [("struct_size", c_size_t), ("q", c_void_p), ("q_stride", c_int64), ("out", c_void_p), ("rows", c_int32), ("heads", c_int32),
+                ("requests", c_int32), ("layer", c_int32)] + \
+               [(name, c_void_p) for name in ("slots", "starts", "offsets", "parents")] + \
+               [("scale", c_float), ("window", c_int32), ("max_nodes", c_int32), ("max_context", c_int32)]
+
+
 DESCRIBE_FN = ctypes.CFUNCTYPE(c_void_p, c_void_p)
 LOAD_FN = ctypes.CFUNCTYPE(c_int32, c_void_p, c_int32, P(c_char_p), P(TensorView))
 FORWARD_FN = ctypes.CFUNCTYPE(c_int32, c_void_p, P(ForwardArgs))
@@ -167,6 +186,12 @@ def lib() -> ctypes.CDLL:
     sig("celeg_check_folder", c_int, c_char_p)
     sig("celeg_check_folder_strict", c_int, c_char_p, c_int32)
     sig("celeg_registered", c_char_p, c_char_p)
+    sig("celeg_token_logprobs_workspace", c_int, P(TokenLogprobsArgs), P(c_size_t))
+    sig("celeg_token_logprobs", c_int, P(TokenLogprobsArgs), c_void_p, c_size_t, c_void_p)
+    sig("celeg_tree_attention_workspace", c_int, P(TreeAttentionArgs), P(PagedCacheStruct), P(c_size_t))
+    sig("celeg_tree_attention", c_int, P(TreeAttentionArgs), P(PagedCacheStruct), c_void_p, c_size_t, c_void_p)
+    sig("celeg_move_tokens", c_int, P(PagedCacheStruct), c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p)
+    sig("celeg_copy_pages", c_int, P(PagedCacheStruct), c_void_p, c_void_p, c_int32, c_void_p)
     sig("celeg_host_new", ctypes.c_longlong, c_char_p, c_char_p)
     sig("celeg_host_call", c_char_p, ctypes.c_longlong, c_char_p, c_char_p)
     sig("celeg_host_delete", None, ctypes.c_longlong)
