@@ -25,32 +25,42 @@ void check_cache(const KVView& kv) {
 }  // namespace
 
 // ---------------------------------------------------------------------------- log probabilities
-static void check(const TokenLogprobs& a) {
+static void check_sizes(const TokenLogprobs& a) {
     floats(a.dtype, "token_logprobs: logits must be float32 or bfloat16");
     need(a.rows >= 0 && a.rows < (1LL << 31), "token_logprobs: the number of rows must be in [0, 2^31)");
     need(a.vocab > 0 && a.vocab <= (1LL << 24), "token_logprobs: the vocabulary must be in [1, 2^24]");
+    need(a.rows * (a.vocab / 8192 + 2) < (1LL << 31), "token_logprobs: too many logits for one call");
     need(a.per_row >= 0 && a.per_row <= TokenLogprobs::MAX_PER_ROW, "token_logprobs: up to 8 tokens a row");
     need(a.top >= 0 && a.top <= TokenLogprobs::MAX_TOP && a.top <= a.vocab, "token_logprobs: top must be in [0, 128] and not above the vocabulary");
     need(a.row_stride >= 0 && (a.rows <= 1 || a.row_stride == 0 || a.row_stride >= a.vocab),
          "token_logprobs: rows must not overlap in part (a row stride of 0 or at least the vocabulary)");
+}
+
+static void check(const TokenLogprobs& a) {
+    check_sizes(a);
     if (a.rows == 0) return;
     need(a.logits != nullptr, "token_logprobs: the logits are missing");
     need(a.per_row == 0 || (a.tokens && a.logprobs && a.ranks), "token_logprobs: tokens, logprobs and ranks come together");
     need(a.top == 0 || (a.top_ids && a.top_logprobs), "token_logprobs: top_ids and top_logprobs are missing");
 }
 
+static void check_workspace(const void* workspace, size_t bytes, size_t needed) {
+    if (!needed) return;
+    need(workspace && bytes >= needed, "the workspace is missing or smaller than the size asked for it");
+    need(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "the workspace must lie on a boundary of 16 bytes");
+}
+
 size_t token_logprobs_workspace(const TokenLogprobs& a) {
-    (void)a;
-    return 0;
+    check_sizes(a);
+    return a.rows ? celeg_logprobs_workspace(static_cast<int>(a.dtype), a.rows, static_cast<int>(a.vocab), a.per_row, a.top) : 0;
 }
 
 void token_logprobs(const TokenLogprobs& a, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     check(a);
-    (void)workspace;
-    (void)workspace_bytes;
     if (a.rows == 0) return;
+    check_workspace(workspace, workspace_bytes, token_logprobs_workspace(a));
     kernel_check(celeg_logprobs_rows(a.logits, static_cast<int>(a.dtype), a.rows, static_cast<int>(a.vocab), a.row_stride, a.tokens,
-                                     a.per_row, a.top, a.logprobs, a.ranks, a.entropy, a.top_ids, a.top_logprobs, stream),
+                                     a.per_row, a.top, a.logprobs, a.ranks, a.entropy, a.top_ids, a.top_logprobs, workspace, stream),
                  "token_logprobs");
 }
 

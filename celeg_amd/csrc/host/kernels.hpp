@@ -267,8 +267,10 @@ int celeg_channel_scan(const float* qk, const float* v, const float* decay, cons
                        size_t state_stride, const int* cu_seqlens, const int* seq_slot, float* out, int n_seqs, int G, int H, int D,
                        int V, int general, hipStream_t stream);
 // token_logprobs.hip
+size_t celeg_logprobs_workspace(int dtype, long long rows, int vocab, int per_row, int top);
 int celeg_logprobs_rows(const void* logits, int dtype, long long rows, int vocab, long long row_stride, const int* tokens, int per_row,
-                        int top, float* logprobs, int* ranks, float* entropy, int* top_ids, float* top_logprobs, hipStream_t stream);
+                        int top, float* logprobs, int* ranks, float* entropy, int* top_ids, float* top_logprobs, void* workspace,
+                        hipStream_t stream);
 // tree_attention.hip
 int celeg_tree_attention_general(const void* q, int ldq, int dtype, const void* k_pool, const void* v_pool, int n_pages, int n_layers,
                                  int layer, int heads, int kv_heads, int head_dim, int page_tokens, const int* table, int table_rows,
