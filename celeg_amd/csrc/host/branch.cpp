@@ -1,5 +1,6 @@
 #include "branch.hpp"
 
+#include <algorithm>
 #include <cmath>
 
 #include "kernels.hpp"
@@ -21,6 +22,11 @@ void check_cache(const KVView& kv) {
     need((kv.v_head_dim > 0) == (kv.v != nullptr), "cache: values and their width come together (keys only: neither)");
     need(static_cast<long long>(kv.table_stride) * kv.page_tokens < (1LL << 31) - 4096, "cache: a request's places must fit 31 bits");
     need(static_cast<long long>(kv.n_layers) * kv.kv_heads <= 65535, "cache: more than 65,535 layers times heads");
+}
+void check_workspace(const void* workspace, size_t bytes, size_t needed) {
+    if (!needed) return;
+    need(workspace && bytes >= needed, "the workspace is missing or smaller than the size asked for it");
+    need(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "the workspace must lie on a boundary of 16 bytes");
 }
 }  // namespace
 
@@ -44,12 +50,6 @@ static void check(const TokenLogprobs& a) {
     need(a.top == 0 || (a.top_ids && a.top_logprobs), "token_logprobs: top_ids and top_logprobs are missing");
 }
 
-static void check_workspace(const void* workspace, size_t bytes, size_t needed) {
-    if (!needed) return;
-    need(workspace && bytes >= needed, "the workspace is missing or smaller than the size asked for it");
-    need(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "the workspace must lie on a boundary of 16 bytes");
-}
-
 size_t token_logprobs_workspace(const TokenLogprobs& a) {
     check_sizes(a);
     return a.rows ? celeg_logprobs_workspace(static_cast<int>(a.dtype), a.rows, static_cast<int>(a.vocab), a.per_row, a.top) : 0;
@@ -65,7 +65,7 @@ void token_logprobs(const TokenLogprobs& a, void* workspace, size_t workspace_by
 }
 
 // ---------------------------------------------------------------------------- attention of trees
-static void check(const TreeAttention& a, const KVView& kv) {
+static void check_sizes(const TreeAttention& a, const KVView& kv) {
     check_cache(kv);
     need(kv.v_head_dim == kv.head_dim, "tree_attention: values of the keys' width only");
     need(kv.layer >= 0 && kv.layer < kv.n_layers, "tree_attention: layer outside the cache");
@@ -79,21 +79,44 @@ static void check(const TreeAttention& a, const KVView& kv) {
     const long long width = static_cast<long long>(a.heads) * kv.head_dim;
     need(a.rows <= 1 || a.q_stride >= width, "tree_attention: the rows of q overlap");
     need(a.q_stride >= 0 && a.q_stride < (1LL << 31), "tree_attention: the row stride of q must be in [0, 2^31)");
+}
+
+static void check(const TreeAttention& a, const KVView& kv) {
+    check_sizes(a, kv);
     if (a.rows == 0 || a.requests == 0) return;
     need(a.q && a.out && a.slots && a.starts && a.offsets && a.parents, "tree_attention: an argument is missing");
 }
 
+// Parts that the contexts are cut into, 0: the kernel for any sizes, which reads single values.
+static int tree_parts(const TreeAttention& a, const KVView& kv) {
+    const uintptr_t low = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(kv.k) |
+                          reinterpret_cast<uintptr_t>(kv.v) | (a.rows > 1 ? static_cast<uintptr_t>(a.q_stride) * dtype_size(kv.dtype) : 0);
+    if (low % 16 || !celeg_tree_attention_fast_ok(kv.head_dim, kv.page_tokens)) return 0;
+    const long long room = static_cast<long long>(kv.table_stride) * kv.page_tokens;
+    const int context = static_cast<int>(a.max_context > 0 ? std::min<long long>(a.max_context, room) : room);
+    return celeg_tree_attention_parts(static_cast<int>(kv.dtype), kv.head_dim, a.requests, kv.kv_heads, a.heads / kv.kv_heads, a.max_nodes, context);
+}
+
 size_t tree_attention_workspace(const TreeAttention& a, const KVView& kv) {
-    (void)a;
-    (void)kv;
-    return 0;
+    check_sizes(a, kv);
+    if (a.rows == 0 || a.requests == 0) return 0;
+    const int parts = tree_parts(a, kv);
+    return parts > 1 ? static_cast<size_t>(a.rows) * a.heads * parts * (kv.head_dim + 2) * sizeof(float) : 0;
 }
 
 void tree_attention(const TreeAttention& a, const KVView& kv, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     check(a, kv);
-    (void)workspace;
-    (void)workspace_bytes;
     if (a.rows == 0 || a.requests == 0) return;
+    check_workspace(workspace, workspace_bytes, tree_attention_workspace(a, kv));
+    const int parts = tree_parts(a, kv);
+    if (parts > 0) {
+        kernel_check(celeg_tree_attention_fast(a.q, static_cast<int>(a.q_stride), static_cast<int>(kv.dtype), kv.k, kv.v, kv.n_pages,
+                                               kv.n_layers, kv.layer, a.heads, kv.kv_heads, kv.head_dim, kv.page_tokens, kv.table,
+                                               kv.table_rows, kv.table_stride, a.slots, a.starts, a.offsets, a.parents, a.requests, a.rows,
+                                               a.max_nodes, parts, a.scale, a.window, a.out, workspace, stream),
+                     "tree_attention (matrix cores)");
+        return;
+    }
     kernel_check(celeg_tree_attention_general(a.q, static_cast<int>(a.q_stride), static_cast<int>(kv.dtype), kv.k, kv.v, kv.n_pages,
                                               kv.n_layers, kv.layer, a.heads, kv.kv_heads, kv.head_dim, kv.page_tokens, kv.table,
                                               kv.table_rows, kv.table_stride, a.slots, a.starts, a.offsets, a.parents, a.requests, a.rows,

@@ -272,6 +272,12 @@ int celeg_logprobs_rows(const void* logits, int dtype, long long rows, int vocab
                         int top, float* logprobs, int* ranks, float* entropy, int* top_ids, float* top_logprobs, void* workspace,
                         hipStream_t stream);
 // tree_attention.hip
+int celeg_tree_attention_fast_ok(int head_dim, int page_tokens);
+int celeg_tree_attention_parts(int dtype, int head_dim, int requests, int kv_heads, int group, int max_nodes, int max_context);
+int celeg_tree_attention_fast(const void* q, int ldq, int dtype, const void* k_pool, const void* v_pool, int n_pages, int n_layers, int layer,
+                              int heads, int kv_heads, int head_dim, int page_tokens, const int* table, int table_rows, int table_stride,
+                              const int* slots, const int* starts, const int* offsets, const int* parents, int n_requests, int n_rows,
+                              int max_nodes, int parts, float scale, int window, void* out, void* workspace, hipStream_t stream);
 int celeg_tree_attention_general(const void* q, int ldq, int dtype, const void* k_pool, const void* v_pool, int n_pages, int n_layers,
                                  int layer, int heads, int kv_heads, int head_dim, int page_tokens, const int* table, int table_rows,
                                  int table_stride, const int* slots, const int* starts, const int* offsets, const int* parents,

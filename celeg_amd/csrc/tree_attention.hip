@@ -5,11 +5,19 @@
 // window w) the keys at positions above its own less w.  out = softmax(scale q . k) v over what it sees.
 // parents[row]: the index inside its request's tree of a node's parent; what is not an index below the node's own makes it a root.
 //   K [pages, layers, kv_heads, page_tokens, head_dim], V [pages, layers, kv_heads, head_dim, page_tokens]
+//
+// The query heads that share a key/value head, for all nodes of a tree, are the rows of matrix instructions: every key and value is
+// asked for once for up to 64 rows.  A workgroup's four wavefronts take rounds of keys in turn, each with a running maximum,
+// sum and output of its own, and meet in LDS; long contexts are cut into parts for as many workgroups, which a second kernel joins.
 #include "common.h"
+#include <algorithm>
 
 #define TREE_MAX_NODES 256
 
-// What a key outside the tree or an ancestor is to a node: all arguments in places, positions and depths.
+typedef __bf16 tree_bf16x8 __attribute__((ext_vector_type(8)));
+typedef float tree_f4 __attribute__((ext_vector_type(4)));
+typedef unsigned int tree_u4 __attribute__((ext_vector_type(4)));
+
 __device__ __forceinline__ int tree_depth(const int* parents, int node) {
     int depth = 0;
     for (int at = node;;) {
@@ -18,6 +26,487 @@ __device__ __forceinline__ int tree_depth(const int* parents, int node) {
         at = up;
         ++depth;
     }
+}
+
+// ---------------------------------------------------------------------------- on the matrix cores
+struct TreeArgs {
+    const void* q;
+    const void* k_pool;
+    const void* v_pool;
+    const int* table;
+    const int *slots, *starts, *offsets, *parents;
+    void* out;
+    float* ws_o;                 // [rows, heads, parts, head_dim]: outputs of parts, not divided
+    float* ws_ml;                // [rows, heads, parts, 2]: their maximum (in powers of two) and sum
+    int ldq, n_pages, n_layers, layer, heads, kv_heads, group, page_tokens, page_shift, table_rows, table_stride, requests, n_rows, max_nodes;
+    int parts, row_blocks, units;      // units: requests * kv_heads * parts
+    float scale;                 // times log2(e)
+    int window;
+};
+
+// How keys and values lie in the operands.  A round holds KEYS keys; `a` of a key tile is 16 keys by the head's values, a
+// lane's (c, qd) = (lane % 16, lane / 16) share of it key KEY(tile, c); a score tile leaves a lane the scores of row c with the four
+// keys FIRST(tile, qd) .. + 3 of the round, which are in turn the keys that it has to hold of the values.
+template <typename T, int HD> struct TreeOps;
+
+template <int HD> struct TreeOps<bf16, HD> {
+    static constexpr int KEYS = HD <= 64 ? 64 : 32, TILES = KEYS / 16, KS = HD / 32, DT = HD / 16, VG = KEYS / 32, VKEYS = 8;
+    typedef tree_bf16x8 Frag;
+    static __device__ __forceinline__ int key(int tile, int c) { return 32 * (tile >> 1) + 8 * (c >> 2) + 4 * (tile & 1) + (c & 3); }
+    static __device__ __forceinline__ int first(int tile, int qd) { return 32 * (tile >> 1) + 8 * qd + 4 * (tile & 1); }
+    static __device__ __forceinline__ int vkey(int g, int qd) { return 32 * g + 8 * qd; }
+    static __device__ __forceinline__ int dim(int s, int qd) { return 32 * s + 8 * qd; }
+    static __device__ __forceinline__ tree_f4 scores(const Frag (&k)[KS], const Frag (&q)[KS]) {
+        tree_f4 acc = tree_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[s], q[s], acc, 0, 0, 0);
+        return acc;
+    }
+    // o += V^T p; the weights enter rounded to bfloat16 (half a step, 2^-8 of each; the sum l is taken of the exact ones)
+    static __device__ __forceinline__ void values(const Frag (&v)[DT][VG], const tree_f4 (&p)[TILES], tree_f4 (&o)[DT]) {
+#pragma unroll
+        for (int g = 0; g < VG; ++g) {
+            Frag b;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                b[i] = static_cast<__bf16>(p[2 * g][i]);
+                b[4 + i] = static_cast<__bf16>(p[2 * g + 1][i]);
+            }
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[dt][g], b, o[dt], 0, 0, 0);
+        }
+    }
+    // a bit for every half word whose exponent is all ones (infinities and NaN), and the same with them made 0
+    static __device__ __forceinline__ unsigned not_finite(const Frag& f) {
+        const tree_u4 u = __builtin_bit_cast(tree_u4, f);
+        unsigned bad = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bad |= ((u[e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+        return bad;
+    }
+    static __device__ __forceinline__ void make_finite(Frag& f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float x = static_cast<float>(f[e]);
+            if (!(fabsf(x) < INFINITY)) f[e] = static_cast<__bf16>(0.f);
+        }
+    }
+};
+
+template <int HD> struct TreeOps<float, HD> {
+    static constexpr int KEYS = 32, TILES = KEYS / 16, KS = HD / 16, DT = HD / 16, VG = TILES, VKEYS = 4;
+    typedef tree_f4 Frag;
+    static __device__ __forceinline__ int key(int tile, int c) { return 16 * tile + c; }
+    static __device__ __forceinline__ int first(int tile, int qd) { return 16 * tile + 4 * qd; }
+    static __device__ __forceinline__ int vkey(int g, int qd) { return 16 * g + 4 * qd; }
+    // (a product sums over the head's values in any order: a lane holds a quarter of them that lie side by side)
+    static __device__ __forceinline__ int dim(int s, int qd) { return (HD / 4) * qd + 4 * s; }
+    static __device__ __forceinline__ tree_f4 scores(const Frag (&k)[KS], const Frag (&q)[KS]) {
+        tree_f4 acc = tree_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][e], q[s][e], acc, 0, 0, 0);
+        return acc;
+    }
+    static __device__ __forceinline__ void values(const Frag (&v)[DT][VG], const tree_f4 (&p)[TILES], tree_f4 (&o)[DT]) {
+#pragma unroll
+        for (int g = 0; g < VG; ++g)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) o[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[dt][g][i], p[g][i], o[dt], 0, 0, 0);
+    }
+    static __device__ __forceinline__ unsigned not_finite(const Frag& f) {
+        unsigned bad = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bad |= !(fabsf(f[e]) < INFINITY);
+        return bad;
+    }
+    static __device__ __forceinline__ void make_finite(Frag& f) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (!(fabsf(f[e]) < INFINITY)) f[e] = 0.f;
+    }
+};
+
+// The keys of a round of 64 from place `base` on that a node sees, a bit each: of the context those from `low` on, of the tree those
+// that the node's words name.
+__device__ __forceinline__ unsigned long long tree_visible(int base, int start, int low, const unsigned long long (&words)[TREE_MAX_NODES / 64]) {
+    const int off = base - start;
+    unsigned long long seen = 0ull;
+    if (off < 0) {
+        const int context = min(-off, 64);
+        seen = context == 64 ? ~0ull : (1ull << context) - 1ull;
+        const int before = low - base;
+        if (before > 0) seen = before >= 64 ? 0ull : seen & (~0ull << before);
+        if (context < 64) seen |= words[0] << context;
+    } else {
+#pragma unroll
+        for (int w = 0; w < TREE_MAX_NODES / 64; ++w) {
+            if ((off >> 6) == w) seen |= words[w] >> (off & 63);
+            if ((off >> 6) + 1 == w && (off & 63)) seen |= words[w] << (64 - (off & 63));
+        }
+    }
+    return seen;
+}
+
+template <typename T, int HD, int RT>
+__global__ __launch_bounds__(256) void tree_attention_kernel(const TreeArgs a) {
+    using O = TreeOps<T, HD>;
+    using Frag = typename O::Frag;
+    constexpr int KEYS = O::KEYS, TILES = O::TILES, KS = O::KS, DT = O::DT, VG = O::VG, WORDS = TREE_MAX_NODES / 64, ROWS = 16 * RT;
+    __shared__ int up[TREE_MAX_NODES];
+    __shared__ unsigned long long words_of[ROWS][WORDS];
+    __shared__ int low_of[ROWS];
+    __shared__ __align__(16) float join_o[2][ROWS][HD];
+    __shared__ float join_ml[2][ROWS][2];
+    // row blocks of the same keys lie a multiple of 8 workgroups apart: on one die, whose cache then holds the keys for all of them
+    const int spread = (a.units + 7) & ~7, block = blockIdx.x / spread, unit = blockIdx.x % spread;
+    if (unit >= a.units) return;
+    const int kvh = unit % a.kv_heads, part = unit / a.kv_heads % a.parts, r = unit / (a.kv_heads * a.parts);
+    const int first = a.offsets[r], count = min(min(a.offsets[r + 1], a.n_rows) - first, a.max_nodes);
+    const int slot = a.slots[r], start = max(a.starts[r], 0);
+    const int rows = count * a.group, j0 = block * ROWS;
+    if (first < 0 || count <= 0 || j0 >= rows || slot < 0 || slot >= a.table_rows) return;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 15, qd = lane >> 4;
+    // (places behind what the table holds are seen by nobody)
+    const int room = a.table_stride << a.page_shift, end = min(start + count, room);
+    const int* __restrict__ pages = a.table + static_cast<size_t>(slot) * a.table_stride;
+    const T* __restrict__ k_pool = static_cast<const T*>(a.k_pool);
+    const T* __restrict__ v_pool = static_cast<const T*>(a.v_pool);
+    const size_t per_head = static_cast<size_t>(HD) << a.page_shift, page_size = per_head * a.kv_heads * a.n_layers;
+    const size_t head_block = per_head * (static_cast<size_t>(a.layer) * a.kv_heads + kvh);
+    const int page_mask = a.page_tokens - 1;
+
+    // ---- the rows' queries, their ways up the tree, and from where on they see the context
+    Frag q[RT][KS];
+    int row_node[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const int j = min(j0 + 16 * t + c, rows - 1), node = j / a.group;
+        row_node[t] = node;
+        const T* from = static_cast<const T*>(a.q) + static_cast<size_t>(first + node) * a.ldq +
+                        static_cast<size_t>(kvh * a.group + j % a.group) * HD;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) q[t][s] = *reinterpret_cast<const Frag*>(from + O::dim(s, qd));
+    }
+    const int n0 = j0 / a.group, n1 = min(j0 + ROWS - 1, rows - 1) / a.group;      // the block's nodes
+    for (int i = tid; i < count; i += 256) up[i] = a.parents[first + i];
+    __syncthreads();
+    if (tid <= n1 - n0) {
+        unsigned long long words[WORDS] = {};
+        int depth = 0;
+        for (int at = n0 + tid;;) {
+#pragma unroll
+            for (int w = 0; w < WORDS; ++w)
+                if ((at >> 6) == w && (a.window <= 0 || depth < a.window)) words[w] |= 1ull << (at & 63);
+            const int next = up[at];
+            if (next < 0 || next >= at) break;         // (indices fall, so the way ends)
+            at = next;
+            ++depth;
+        }
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) words_of[tid][w] = words[w];
+        low_of[tid] = a.window > 0 ? max(0, start + depth - a.window + 1) : 0;
+    }
+    __syncthreads();
+
+    // ---- the part's rounds.  In those from `plain` to `tree` every row sees every key (as long as all pages are there).
+    const int first_round = a.window > 0 ? max(0, start - a.window + 1) / KEYS : 0, last_round = end > 0 ? (end - 1) / KEYS : -1;
+    const int total = last_round - first_round + 1, per = (total + a.parts - 1) / a.parts;
+    const int r_begin = first_round + part * per, r_end = min(last_round, r_begin + per - 1);
+    const int plain = a.window > 0 ? max(0, start + count - a.window) : 0;
+    float m[RT], l[RT];
+    tree_f4 o[RT][DT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        m[t] = -INFINITY;
+        l[t] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[t][dt] = tree_f4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int round = r_begin + wave; round <= r_end; round += 4) {
+        const int base = round * KEYS, top = min(base + KEYS, end) - 1;
+        const int first_page = base >> a.page_shift, last_page = top >> a.page_shift;
+        int page = pages[min(first_page + lane, last_page)];
+        const bool there = page >= 0 && page < a.n_pages;
+        const bool all_there = __ballot(!there) == 0ull;
+        page = there ? page : 0;
+        Frag k[TILES][KS], v[DT][VG];
+#pragma unroll
+        for (int tile = 0; tile < TILES; ++tile) {
+            const int key = min(base + O::key(tile, c), top);
+            const T* from = k_pool + __shfl(page, (key >> a.page_shift) - first_page, 64) * page_size + head_block +
+                            static_cast<size_t>(key & page_mask) * HD;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) k[tile][s] = *reinterpret_cast<const Frag*>(from + O::dim(s, qd));
+        }
+#pragma unroll
+        for (int g = 0; g < VG; ++g) {
+            const int key = min(base + O::vkey(g, qd), top & ~(O::VKEYS - 1));
+            const T* from = v_pool + __shfl(page, (key >> a.page_shift) - first_page, 64) * page_size + head_block + (key & page_mask);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+                v[dt][g] = *reinterpret_cast<const Frag*>(from + (static_cast<size_t>(16 * dt + c) << a.page_shift));
+        }
+        const bool masked = base < plain || base + KEYS > start || !all_there;
+        bool odd_values = false;
+        if (masked) {
+            // A weight of 0 times an infinity or a NaN is no 0: such values are taken out here and added below, for the rows that
+            // see them
+            unsigned bad = 0;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int g = 0; g < VG; ++g) bad |= O::not_finite(v[dt][g]);
+            odd_values = __ballot(bad != 0) != 0ull;
+            if (odd_values) {
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int g = 0; g < VG; ++g) O::make_finite(v[dt][g]);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            tree_f4 s[TILES];
+#pragma unroll
+            for (int tile = 0; tile < TILES; ++tile) s[tile] = O::scores(k[tile], q[t]);
+            unsigned long long seen = ~0ull;
+            if (masked) {
+                unsigned long long words[WORDS];
+#pragma unroll
+                for (int w = 0; w < WORDS; ++w) words[w] = words_of[row_node[t] - n0][w];
+                seen = tree_visible(base, start, low_of[row_node[t] - n0], words);
+                if (base + 64 > end) seen &= end > base ? (1ull << (end - base)) - 1ull : 0ull;
+                if (!all_there) {
+                    for (int i = 0; i < KEYS; i += min(a.page_tokens, KEYS)) {
+                        const int gone = __shfl(static_cast<int>(!there), min((base + i) >> a.page_shift, last_page) - first_page, 64);
+                        const int n = min(a.page_tokens, KEYS);
+                        if (gone) seen &= ~((n == 64 ? ~0ull : (1ull << n) - 1ull) << i);
+                    }
+                }
+#pragma unroll
+                for (int tile = 0; tile < TILES; ++tile)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool sees = (seen >> (O::first(tile, qd) + i)) & 1ull;
+                        s[tile][i] = sees ? s[tile][i] * a.scale : -INFINITY;
+                    }
+            } else {
+#pragma unroll
+                for (int tile = 0; tile < TILES; ++tile) s[tile] *= a.scale;
+            }
+            float high = s[0][0];
+#pragma unroll
+            for (int tile = 0; tile < TILES; ++tile)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) high = fmaxf(high, s[tile][i]);
+            high = max_half32(max_row16(high));
+            // The maximum follows the scores only when some row's grows by more than 8 (a factor 2^8): until then the weights are
+            // taken against the older one, and numerator and denominator carry the same factor.
+            if (__ballot(high > m[t] + 8.f) != 0ull) {
+                const float now = fmaxf(m[t], high);
+                const float keep = m[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[t] - now);
+                m[t] = now;
+                l[t] *= keep;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) o[t][dt] *= keep;
+            }
+            const float shift = m[t] == -INFINITY ? 0.f : m[t];
+#pragma unroll
+            for (int tile = 0; tile < TILES; ++tile)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[tile][i] = __builtin_amdgcn_exp2f(s[tile][i] - shift);
+                    l[t] += s[tile][i];                 // (a lane's own keys; the four lanes of a row meet at the end)
+                }
+            O::values(v, s, o[t]);
+            if (odd_values) {
+                for (int i = 0; i < KEYS; ++i) {
+                    if (!__ballot((seen >> i) & 1ull)) continue;
+                    const int key = base + i;
+                    const T* from = v_pool + __shfl(page, min(key >> a.page_shift, last_page) - first_page, 64) * page_size + head_block +
+                                    (key & page_mask);
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float x = to_float(from[static_cast<size_t>(16 * dt + 4 * qd + e) << a.page_shift]);
+                            if (((seen >> i) & 1ull) && !(fabsf(x) < INFINITY)) o[t][dt][e] += x;
+                        }
+                }
+            }
+        }
+    }
+    // ---- the four wavefronts' results: the upper two to the lower two, then those
+#pragma unroll
+    for (int t = 0; t < RT; ++t) l[t] = sum_half32(sum_row16(l[t]));
+    for (int half = 2; half >= 1; half >>= 1) {
+        if (wave >= half && wave < 2 * half) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                if (qd == 0) {
+                    join_ml[wave - half][16 * t + c][0] = m[t];
+                    join_ml[wave - half][16 * t + c][1] = l[t];
+                }
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<tree_f4*>(&join_o[wave - half][16 * t + c][16 * dt + 4 * qd]) = o[t][dt];
+            }
+        }
+        __syncthreads();
+        if (wave < half) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                const float other = join_ml[wave][16 * t + c][0], now = fmaxf(m[t], other), shift = now == -INFINITY ? 0.f : now;
+                const float mine = __builtin_amdgcn_exp2f(m[t] - shift), theirs = __builtin_amdgcn_exp2f(other - shift);
+                l[t] = l[t] * mine + join_ml[wave][16 * t + c][1] * theirs;
+                m[t] = now;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+                    o[t][dt] = o[t][dt] * mine + *reinterpret_cast<const tree_f4*>(&join_o[wave][16 * t + c][16 * dt + 4 * qd]) * theirs;
+            }
+        }
+        __syncthreads();
+    }
+    if (wave != 0) return;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const int j = j0 + 16 * t + c;
+        if (j >= rows) continue;
+        const size_t row = first + row_node[t], head = kvh * a.group + j % a.group;
+        if (a.parts == 1) {
+            T* to = static_cast<T*>(a.out) + (row * a.heads + head) * HD + 4 * qd;
+            const float inverse = 1.f / l[t];
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const float x[4] = {o[t][dt][0] * inverse, o[t][dt][1] * inverse, o[t][dt][2] * inverse, o[t][dt][3] * inverse};
+                Vec4<T>::store(to + 16 * dt, x);
+            }
+        } else {
+            const size_t at = (row * a.heads + head) * a.parts + part;
+            if (qd == 0) {
+                a.ws_ml[2 * at] = m[t];
+                a.ws_ml[2 * at + 1] = l[t];
+            }
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<tree_f4*>(a.ws_o + at * HD + 16 * dt + 4 * qd) = o[t][dt];
+        }
+    }
+}
+
+// The parts of a node and query head: out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.  A wavefront each; four to a workgroup.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void tree_join_kernel(const TreeArgs a) {
+    const int lane = threadIdx.x & 63;
+    const long long id = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int head = static_cast<int>(id % a.heads), node = static_cast<int>(id / a.heads % a.max_nodes);
+    const long long r = id / (static_cast<long long>(a.heads) * a.max_nodes);
+    if (r >= a.requests) return;
+    const int first = a.offsets[r], count = min(a.offsets[r + 1], a.n_rows) - first, slot = a.slots[r];
+    if (first < 0 || node >= count || slot < 0 || slot >= a.table_rows) return;
+    const size_t at = (static_cast<size_t>(first + node) * a.heads + head) * a.parts;
+    float high = -INFINITY;
+    for (int p = lane; p < a.parts; p += 64) high = fmaxf(high, a.ws_ml[2 * (at + p)]);
+    high = wave_max(high);
+    const float shift = high == -INFINITY ? 0.f : high;
+    constexpr int PER = (HD + 63) / 64;
+    float sum = 0.f, o[PER] = {};
+    for (int p = 0; p < a.parts; ++p) {
+        const float w = __builtin_amdgcn_exp2f(a.ws_ml[2 * (at + p)] - shift);
+        sum = fmaf(w, a.ws_ml[2 * (at + p) + 1], sum);
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+            if (lane + 64 * e < HD) o[e] = fmaf(w, a.ws_o[(at + p) * HD + lane + 64 * e], o[e]);
+    }
+    T* to = static_cast<T*>(a.out) + (static_cast<size_t>(first + node) * a.heads + head) * HD;
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+        if (lane + 64 * e < HD) to[lane + 64 * e] = from_float<T>(o[e] / sum);
+}
+
+// Rows a workgroup takes (16 times this) and keys of a round, for these sizes.
+static int tree_row_tiles(int dtype, int head_dim, int rows) {
+    const int most = dtype == CELEG_BF16 ? (head_dim <= 64 ? 4 : 2) : (head_dim <= 64 ? 2 : 1);
+    return rows <= 16 ? 1 : rows <= 32 || most == 2 ? std::min(2, most) : most;
+}
+static int tree_round_keys(int dtype, int head_dim) { return dtype == CELEG_BF16 && head_dim <= 64 ? 64 : 32; }
+
+// Whether the matrix cores take these sizes.
+extern "C" int celeg_tree_attention_fast_ok(int head_dim, int page_tokens) {
+    return (head_dim == 32 || head_dim == 64 || head_dim == 96 || head_dim == 128) && page_tokens >= 16 && (page_tokens & (page_tokens - 1)) == 0;
+}
+
+// Parts that the contexts are cut into: about two workgroups a compute unit, each wavefront with a round at least.
+extern "C" int celeg_tree_attention_parts(int dtype, int head_dim, int requests, int kv_heads, int group, int max_nodes, int max_context) {
+    const int rows = max_nodes * group, block = 16 * tree_row_tiles(dtype, head_dim, rows), keys = tree_round_keys(dtype, head_dim);
+    const long long groups = static_cast<long long>(requests) * kv_heads * ((rows + block - 1) / block);
+    const long long rounds = (static_cast<long long>(max_context) + max_nodes + keys - 1) / keys;
+    return static_cast<int>(std::max(1LL, std::min({(512 + groups - 1) / groups, (rounds + 3) / 4, 64LL})));
+}
+
+extern "C" int celeg_tree_attention_fast(const void* q, int ldq, int dtype, const void* k_pool, const void* v_pool, int n_pages, int n_layers,
+                                         int layer, int heads, int kv_heads, int head_dim, int page_tokens, const int* table, int table_rows,
+                                         int table_stride, const int* slots, const int* starts, const int* offsets, const int* parents,
+                                         int n_requests, int n_rows, int max_nodes, int parts, float scale, int window, void* out,
+                                         void* workspace, hipStream_t stream) {
+    TreeArgs a;
+    a.q = q;
+    a.k_pool = k_pool;
+    a.v_pool = v_pool;
+    a.table = table;
+    a.slots = slots;
+    a.starts = starts;
+    a.offsets = offsets;
+    a.parents = parents;
+    a.out = out;
+    a.ws_o = static_cast<float*>(workspace);
+    a.ws_ml = parts > 1 ? a.ws_o + static_cast<size_t>(n_rows) * heads * parts * head_dim : nullptr;
+    a.ldq = ldq;
+    a.n_pages = n_pages;
+    a.n_layers = n_layers;
+    a.layer = layer;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.group = heads / kv_heads;
+    a.page_tokens = page_tokens;
+    a.page_shift = __builtin_ctz(page_tokens);
+    a.table_rows = table_rows;
+    a.table_stride = table_stride;
+    a.requests = n_requests;
+    a.n_rows = n_rows;
+    a.max_nodes = max_nodes;
+    a.parts = parts;
+    a.units = n_requests * kv_heads * parts;
+    a.scale = scale * 1.44269504088896340736f;
+    a.window = window;
+    const int rows = max_nodes * a.group, tiles = tree_row_tiles(dtype, head_dim, rows);
+    a.row_blocks = (rows + 16 * tiles - 1) / (16 * tiles);
+    const dim3 grid(static_cast<unsigned>((a.units + 7) / 8 * 8) * a.row_blocks);
+    const dim3 join(static_cast<unsigned>((static_cast<long long>(n_requests) * max_nodes * heads + 3) / 4));
+    auto run = [&](auto* type, auto dim) {
+        using T = std::remove_pointer_t<decltype(type)>;
+        constexpr int HD = decltype(dim)::value;
+        constexpr bool B = std::is_same<T, bf16>::value;
+        if constexpr ((B && HD <= 64)) {
+            if (tiles == 4) tree_attention_kernel<T, HD, 4><<<grid, dim3(256), 0, stream>>>(a);
+        }
+        if constexpr (B || HD <= 64) {
+            if (tiles == 2) tree_attention_kernel<T, HD, 2><<<grid, dim3(256), 0, stream>>>(a);
+        }
+        if (tiles == 1) tree_attention_kernel<T, HD, 1><<<grid, dim3(256), 0, stream>>>(a);
+        if (parts > 1) tree_join_kernel<T, HD><<<join, dim3(256), 0, stream>>>(a);
+    };
+    auto by_dim = [&](auto* type) {
+        if (head_dim == 32) run(type, std::integral_constant<int, 32>{});
+        else if (head_dim == 64) run(type, std::integral_constant<int, 64>{});
+        else if (head_dim == 96) run(type, std::integral_constant<int, 96>{});
+        else run(type, std::integral_constant<int, 128>{});
+    };
+    if (dtype == CELEG_BF16) by_dim(static_cast<bf16*>(nullptr));
+    else by_dim(static_cast<float*>(nullptr));
+    return CELEG_LAUNCH_RESULT();
 }
 
 // ---------------------------------------------------------------------------- any sizes
