@@ -40,7 +40,8 @@ struct TreeArgs {
     float* ws_ml;                // [rows, heads, parts, 2]: their maximum (in powers of two) and sum
     int ldq, n_pages, n_layers, layer, heads, kv_heads, group, page_tokens, page_shift, table_rows, table_stride, requests, n_rows, max_nodes;
     int parts, row_blocks, units;      // units: requests * kv_heads * parts
-    float scale;                 // times log2(e)
+    float scale;                 // its size times log2(e); `turned`: it is negative, and q enters with the other sign
+    bool turned;
     int window;
 };
 
@@ -76,6 +77,7 @@ template <int HD> struct TreeOps<bf16, HD> {
             for (int dt = 0; dt < DT; ++dt) o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[dt][g], b, o[dt], 0, 0, 0);
         }
     }
+    static __device__ __forceinline__ void turn(Frag& f) { f = __builtin_bit_cast(Frag, __builtin_bit_cast(tree_u4, f) ^ 0x80008000u); }
     // a bit for every half word whose exponent is all ones (infinities and NaN), and the same with them made 0
     static __device__ __forceinline__ unsigned not_finite(const Frag& f) {
         const tree_u4 u = __builtin_bit_cast(tree_u4, f);
@@ -117,6 +119,7 @@ template <int HD> struct TreeOps<float, HD> {
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) o[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[dt][g][i], p[g][i], o[dt], 0, 0, 0);
     }
+    static __device__ __forceinline__ void turn(Frag& f) { f = -f; }
     static __device__ __forceinline__ unsigned not_finite(const Frag& f) {
         unsigned bad = 0;
 #pragma unroll
@@ -151,48 +154,33 @@ __device__ __forceinline__ unsigned long long tree_visible(int base, int start, 
     return seen;
 }
 
-template <typename T, int HD, int RT>
-__global__ __launch_bounds__(256) void tree_attention_kernel(const TreeArgs a) {
-    using O = TreeOps<T, HD>;
-    using Frag = typename O::Frag;
-    constexpr int KEYS = O::KEYS, TILES = O::TILES, KS = O::KS, DT = O::DT, VG = O::VG, WORDS = TREE_MAX_NODES / 64, ROWS = 16 * RT;
-    __shared__ int up[TREE_MAX_NODES];
-    __shared__ unsigned long long words_of[ROWS][WORDS];
-    __shared__ int low_of[ROWS];
-    __shared__ __align__(16) float join_o[2][ROWS][HD];
-    __shared__ float join_ml[2][ROWS][2];
-    // row blocks of the same keys lie a multiple of 8 workgroups apart: on one die, whose cache then holds the keys for all of them
-    const int spread = (a.units + 7) & ~7, block = blockIdx.x / spread, unit = blockIdx.x % spread;
-    if (unit >= a.units) return;
-    const int kvh = unit % a.kv_heads, part = unit / a.kv_heads % a.parts, r = unit / (a.kv_heads * a.parts);
-    const int first = a.offsets[r], count = min(min(a.offsets[r + 1], a.n_rows) - first, a.max_nodes);
-    const int slot = a.slots[r], start = max(a.starts[r], 0);
-    const int rows = count * a.group, j0 = block * ROWS;
-    if (first < 0 || count <= 0 || j0 >= rows || slot < 0 || slot >= a.table_rows) return;
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 15, qd = lane >> 4;
-    // (places behind what the table holds are seen by nobody)
-    const int room = a.table_stride << a.page_shift, end = min(start + count, room);
-    const int* __restrict__ pages = a.table + static_cast<size_t>(slot) * a.table_stride;
-    const T* __restrict__ k_pool = static_cast<const T*>(a.k_pool);
-    const T* __restrict__ v_pool = static_cast<const T*>(a.v_pool);
-    const size_t per_head = static_cast<size_t>(HD) << a.page_shift, page_size = per_head * a.kv_heads * a.n_layers;
-    const size_t head_block = per_head * (static_cast<size_t>(a.layer) * a.kv_heads + kvh);
-    const int page_mask = a.page_tokens - 1;
-
-    // ---- the rows' queries, their ways up the tree, and from where on they see the context
-    Frag q[RT][KS];
-    int row_node[RT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const int j = min(j0 + 16 * t + c, rows - 1), node = j / a.group;
-        row_node[t] = node;
-        const T* from = static_cast<const T*>(a.q) + static_cast<size_t>(first + node) * a.ldq +
-                        static_cast<size_t>(kvh * a.group + j % a.group) * HD;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) q[t][s] = *reinterpret_cast<const Frag*>(from + O::dim(s, qd));
+// The request of a workgroup: which rows and keys it has.  ok: there is something to do.
+struct TreeRequest {
+    int first, count, slot, start, rows, end;
+    bool ok;
+    const int* pages;
+    __device__ __forceinline__ TreeRequest(const TreeArgs& a, int r) {
+        first = a.offsets[r];
+        count = min(min(a.offsets[r + 1], a.n_rows) - first, a.max_nodes);
+        slot = a.slots[r];
+        start = max(a.starts[r], 0);
+        rows = count * a.group;
+        // (places behind what the table holds are seen by nobody)
+        const int room = a.table_stride << a.page_shift;
+        end = start < room ? min(start + count, room) : room;
+        ok = first >= 0 && count > 0 && slot >= 0 && slot < a.table_rows;
+        pages = a.table + static_cast<size_t>(ok ? slot : 0) * a.table_stride;
     }
-    const int n0 = j0 / a.group, n1 = min(j0 + ROWS - 1, rows - 1) / a.group;      // the block's nodes
-    for (int i = tid; i < count; i += 256) up[i] = a.parents[first + i];
+};
+
+// The ways up the tree of the nodes n0 .. n1 (at most as many as threads), and from where on each sees the context; all
+// threads call it, and meet a barrier afterwards.
+template <int THREADS>
+__device__ __forceinline__ void tree_ways(const TreeArgs& a, const TreeRequest& q, int n0, int n1, int* up,
+                                          unsigned long long (*words_of)[TREE_MAX_NODES / 64], int* low_of) {
+    constexpr int WORDS = TREE_MAX_NODES / 64;
+    const int tid = threadIdx.x;
+    for (int i = tid; i < q.count; i += THREADS) up[i] = a.parents[q.first + i];
     __syncthreads();
     if (tid <= n1 - n0) {
         unsigned long long words[WORDS] = {};
@@ -208,15 +196,178 @@ __global__ __launch_bounds__(256) void tree_attention_kernel(const TreeArgs a) {
         }
 #pragma unroll
         for (int w = 0; w < WORDS; ++w) words_of[tid][w] = words[w];
-        low_of[tid] = a.window > 0 ? max(0, start + depth - a.window + 1) : 0;
+        low_of[tid] = a.window > 0 ? max(0, q.start + depth - a.window + 1) : 0;
     }
     __syncthreads();
+}
 
-    // ---- the part's rounds.  In those from `plain` to `tree` every row sees every key (as long as all pages are there).
-    const int first_round = a.window > 0 ? max(0, start - a.window + 1) / KEYS : 0, last_round = end > 0 ? (end - 1) / KEYS : -1;
-    const int total = last_round - first_round + 1, per = (total + a.parts - 1) / a.parts;
-    const int r_begin = first_round + part * per, r_end = min(last_round, r_begin + per - 1);
-    const int plain = a.window > 0 ? max(0, start + count - a.window) : 0;
+// The rounds of a part, r_begin .. r_end.  In those that begin at `plain` or later and end before the tree every row sees every
+// key, as long as all pages are there.
+struct TreeRounds {
+    int r_begin, r_end, plain;
+    __device__ __forceinline__ TreeRounds(const TreeArgs& a, const TreeRequest& q, int part, int keys) {
+        const int first = a.window > 0 ? max(0, q.start - a.window + 1) / keys : 0, last = q.end > 0 ? (q.end - 1) / keys : -1;
+        const int total = max(last - first + 1, 0), per = (total + a.parts - 1) / a.parts;
+        r_begin = first + part * per;
+        r_end = min(last, r_begin + per - 1);
+        plain = a.window > 0 ? max(0, q.start + q.count - a.window) : 0;
+    }
+};
+
+// One row tile's scores of a round into weights, its running maximum m (in powers of two), sum l (a lane's own keys; the four
+// lanes of a row meet at the end) and output o brought up to date.  MASKED: the scores are scaled and hidden ones -inf already.
+// The maximum follows the scores only when some row's grows by more than 8 (a factor 2^8): until then the weights are taken against the
+// older one, and numerator and denominator carry the same factor.
+template <bool MASKED, int TILES, int DT>
+__device__ __forceinline__ void tree_softmax(tree_f4 (&s)[TILES], float& m, float& l, tree_f4 (&o)[DT], float scale) {
+    float high = s[0][0];
+#pragma unroll
+    for (int tile = 0; tile < TILES; ++tile)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) high = fmaxf(high, s[tile][i]);
+    high = max_half32(max_row16(high));
+    if (!MASKED) high *= scale;
+    if (__ballot(high > m + 8.f) != 0ull) {
+        const float now = fmaxf(m, high);
+        const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - now);
+        m = now;
+        l *= keep;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] *= keep;
+    }
+    const float shift = m == -INFINITY ? 0.f : m;
+    float sum = 0.f;
+#pragma unroll
+    for (int tile = 0; tile < TILES; ++tile)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            s[tile][i] = __builtin_amdgcn_exp2f(MASKED ? s[tile][i] - shift : fmaf(s[tile][i], scale, -shift));
+            sum += s[tile][i];
+        }
+    l += sum;
+}
+
+// The keys of the round from `base` on that a row sees, a bit each (page: the lane's page of the round, `gone` if it is none).
+template <int KEYS>
+__device__ __forceinline__ unsigned long long tree_seen(const TreeArgs& a, const TreeRequest& q, int base, bool all_there, bool gone, int last_page,
+                                                        int low, const unsigned long long* words_of) {
+    unsigned long long words[TREE_MAX_NODES / 64];
+#pragma unroll
+    for (int w = 0; w < TREE_MAX_NODES / 64; ++w) words[w] = words_of[w];
+    unsigned long long seen = tree_visible(base, q.start, low, words);
+    if (base + 64 > q.end) seen &= (1ull << (q.end - base)) - 1ull;
+    if (!all_there) {
+        const int n = min(a.page_tokens, KEYS), first_page = base >> a.page_shift;
+        for (int i = 0; i < KEYS; i += n)
+            if (__shfl(static_cast<int>(gone), min((base + i) >> a.page_shift, last_page) - first_page, 64))
+                seen &= ~((n == 64 ? ~0ull : (1ull << n) - 1ull) << i);
+    }
+    return seen;
+}
+
+// What the matrix instructions left out of a round: infinities and NaN among the values, for the rows that see them.
+template <typename T, int KEYS, int DT>
+__device__ __noinline__ void tree_odd_values_of(tree_f4 (&o)[DT], const T* from_head, size_t page_size, int page_shift, int base, int last_page, int page,
+                                             unsigned long long seen) {
+    const int qd = (threadIdx.x & 63) >> 4;
+    for (int i = 0; i < KEYS; ++i) {
+        if (!__ballot((seen >> i) & 1ull)) continue;
+        const int key = base + i;
+        const T* from = from_head + __shfl(page, min(key >> page_shift, last_page) - (base >> page_shift), 64) * page_size +
+                        (key & ((1 << page_shift) - 1));
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = to_float(from[static_cast<size_t>(16 * dt + 4 * qd + e) << page_shift]);
+                if (((seen >> i) & 1ull) && !(fabsf(x) < INFINITY)) o[dt][e] += x;
+            }
+    }
+}
+
+// (a copy goes to the function, so that the outputs themselves stay in registers)
+template <typename T, int KEYS, int DT>
+__device__ __forceinline__ void tree_odd_values(tree_f4 (&o)[DT], const T* from_head, size_t page_size, int page_shift, int base, int last_page,
+                                                int page, unsigned long long seen) {
+    tree_f4 copy[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) copy[dt] = o[dt];
+    tree_odd_values_of<T, KEYS, DT>(copy, from_head, page_size, page_shift, base, last_page, page, seen);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt] = copy[dt];
+}
+
+// A row's result: to `out`, or, where the context is cut, its part's maximum, sum and output to the workspace.
+template <typename T, int HD>
+__device__ __forceinline__ void tree_store(const TreeArgs& a, size_t row, int head, int part, int qd, float m, float l, const tree_f4 (&o)[HD / 16]) {
+    if (a.parts == 1) {
+        T* to = static_cast<T*>(a.out) + (row * a.heads + head) * HD + 4 * qd;
+        const float inverse = 1.f / l;
+#pragma unroll
+        for (int dt = 0; dt < HD / 16; ++dt) {
+            const float x[4] = {o[dt][0] * inverse, o[dt][1] * inverse, o[dt][2] * inverse, o[dt][3] * inverse};
+            Vec4<T>::store(to + 16 * dt, x);
+        }
+    } else {
+        const size_t at = (row * a.heads + head) * a.parts + part;
+        if (qd == 0) {
+            a.ws_ml[2 * at] = m;
+            a.ws_ml[2 * at + 1] = l;
+        }
+#pragma unroll
+        for (int dt = 0; dt < HD / 16; ++dt) *reinterpret_cast<tree_f4*>(a.ws_o + at * HD + 16 * dt + 4 * qd) = o[dt];
+    }
+}
+
+template <typename T, int HD, int RT>
+__device__ __forceinline__ void tree_queries(const TreeArgs& a, const TreeRequest& w, int kvh, int j0, typename TreeOps<T, HD>::Frag (&q)[RT][TreeOps<T, HD>::KS],
+                                             int (&node_of)[RT]) {
+    using O = TreeOps<T, HD>;
+    const int lane = threadIdx.x & 63, c = lane & 15, qd = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const int j = min(j0 + 16 * t + c, w.rows - 1), node = j / a.group;
+        node_of[t] = node;
+        const T* from = static_cast<const T*>(a.q) + static_cast<size_t>(w.first + node) * a.ldq +
+                        static_cast<size_t>(kvh * a.group + j % a.group) * HD;
+#pragma unroll
+        for (int s = 0; s < O::KS; ++s) {
+            q[t][s] = *reinterpret_cast<const typename O::Frag*>(from + O::dim(s, qd));
+            if (a.turned) O::turn(q[t][s]);
+        }
+    }
+}
+
+// ---- few rows: operands straight from memory, the wavefronts take the rounds in turn
+template <typename T, int HD, int RT>
+__global__ __launch_bounds__(256) void tree_few_kernel(const TreeArgs a) {
+    using O = TreeOps<T, HD>;
+    using Frag = typename O::Frag;
+    constexpr int KEYS = O::KEYS, TILES = O::TILES, KS = O::KS, DT = O::DT, VG = O::VG, ROWS = 16 * RT;
+    __shared__ int up[TREE_MAX_NODES];
+    __shared__ unsigned long long words_of[ROWS][TREE_MAX_NODES / 64];
+    __shared__ int low_of[ROWS];
+    __shared__ __align__(16) float join_o[2][ROWS][HD];
+    __shared__ float join_ml[2][ROWS][2];
+    // row blocks of the same keys lie a multiple of 8 workgroups apart: on one die, whose cache then holds the keys for all of them
+    const int spread = (a.units + 7) & ~7, block = blockIdx.x / spread, unit = blockIdx.x % spread;
+    if (unit >= a.units) return;
+    const int kvh = unit % a.kv_heads, part = unit / a.kv_heads % a.parts, r = unit / (a.kv_heads * a.parts);
+    const TreeRequest w(a, r);
+    const int j0 = block * ROWS;
+    if (!w.ok || j0 >= w.rows) return;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 15, qd = lane >> 4;
+    const size_t per_head = static_cast<size_t>(HD) << a.page_shift, page_size = per_head * a.kv_heads * a.n_layers;
+    const size_t head_block = per_head * (static_cast<size_t>(a.layer) * a.kv_heads + kvh);
+    const T* __restrict__ k_pool = static_cast<const T*>(a.k_pool) + head_block;
+    const T* __restrict__ v_pool = static_cast<const T*>(a.v_pool) + head_block;
+    const int page_mask = a.page_tokens - 1;
+    Frag q[RT][KS];
+    int node_of[RT];
+    tree_queries<T, HD, RT>(a, w, kvh, j0, q, node_of);
+    const int n0 = j0 / a.group, n1 = min(j0 + ROWS - 1, w.rows - 1) / a.group;      // the block's nodes
+    tree_ways<256>(a, w, n0, n1, up, words_of, low_of);
+    const TreeRounds rounds(a, w, part, KEYS);
     float m[RT], l[RT];
     tree_f4 o[RT][DT];
 #pragma unroll
@@ -226,10 +377,10 @@ __global__ __launch_bounds__(256) void tree_attention_kernel(const TreeArgs a) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[t][dt] = tree_f4{0.f, 0.f, 0.f, 0.f};
     }
-    for (int round = r_begin + wave; round <= r_end; round += 4) {
-        const int base = round * KEYS, top = min(base + KEYS, end) - 1;
+    for (int round = rounds.r_begin + wave; round <= rounds.r_end; round += 4) {
+        const int base = round * KEYS, top = min(base + KEYS, w.end) - 1;
         const int first_page = base >> a.page_shift, last_page = top >> a.page_shift;
-        int page = pages[min(first_page + lane, last_page)];
+        int page = w.pages[min(first_page + lane, last_page)];
         const bool there = page >= 0 && page < a.n_pages;
         const bool all_there = __ballot(!there) == 0ull;
         page = there ? page : 0;
@@ -237,110 +388,58 @@ __global__ __launch_bounds__(256) void tree_attention_kernel(const TreeArgs a) {
 #pragma unroll
         for (int tile = 0; tile < TILES; ++tile) {
             const int key = min(base + O::key(tile, c), top);
-            const T* from = k_pool + __shfl(page, (key >> a.page_shift) - first_page, 64) * page_size + head_block +
-                            static_cast<size_t>(key & page_mask) * HD;
+            const T* from = k_pool + __shfl(page, (key >> a.page_shift) - first_page, 64) * page_size + static_cast<size_t>(key & page_mask) * HD;
 #pragma unroll
             for (int s = 0; s < KS; ++s) k[tile][s] = *reinterpret_cast<const Frag*>(from + O::dim(s, qd));
         }
 #pragma unroll
         for (int g = 0; g < VG; ++g) {
             const int key = min(base + O::vkey(g, qd), top & ~(O::VKEYS - 1));
-            const T* from = v_pool + __shfl(page, (key >> a.page_shift) - first_page, 64) * page_size + head_block + (key & page_mask);
+            const T* from = v_pool + __shfl(page, (key >> a.page_shift) - first_page, 64) * page_size + (key & page_mask);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
                 v[dt][g] = *reinterpret_cast<const Frag*>(from + (static_cast<size_t>(16 * dt + c) << a.page_shift));
         }
-        const bool masked = base < plain || base + KEYS > start || !all_there;
-        bool odd_values = false;
-        if (masked) {
-            // A weight of 0 times an infinity or a NaN is no 0: such values are taken out here and added below, for the rows that
-            // see them
-            unsigned bad = 0;
+        if (base >= rounds.plain && base + KEYS <= w.start && all_there) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                tree_f4 s[TILES];
+#pragma unroll
+                for (int tile = 0; tile < TILES; ++tile) s[tile] = O::scores(k[tile], q[t]);
+                tree_softmax<false>(s, m[t], l[t], o[t], a.scale);
+                O::values(v, s, o[t]);
+            }
+            continue;
+        }
+        // A weight of 0 times an infinity or a NaN is no 0: such values are taken out, and added for the rows that see them
+        unsigned bad = 0;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int g = 0; g < VG; ++g) bad |= O::not_finite(v[dt][g]);
+        const bool odd_values = __ballot(bad != 0) != 0ull;
+        if (odd_values) {
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                for (int g = 0; g < VG; ++g) bad |= O::not_finite(v[dt][g]);
-            odd_values = __ballot(bad != 0) != 0ull;
-            if (odd_values) {
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                    for (int g = 0; g < VG; ++g) O::make_finite(v[dt][g]);
-            }
+                for (int g = 0; g < VG; ++g) O::make_finite(v[dt][g]);
         }
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
             tree_f4 s[TILES];
 #pragma unroll
             for (int tile = 0; tile < TILES; ++tile) s[tile] = O::scores(k[tile], q[t]);
-            unsigned long long seen = ~0ull;
-            if (masked) {
-                unsigned long long words[WORDS];
-#pragma unroll
-                for (int w = 0; w < WORDS; ++w) words[w] = words_of[row_node[t] - n0][w];
-                seen = tree_visible(base, start, low_of[row_node[t] - n0], words);
-                if (base + 64 > end) seen &= end > base ? (1ull << (end - base)) - 1ull : 0ull;
-                if (!all_there) {
-                    for (int i = 0; i < KEYS; i += min(a.page_tokens, KEYS)) {
-                        const int gone = __shfl(static_cast<int>(!there), min((base + i) >> a.page_shift, last_page) - first_page, 64);
-                        const int n = min(a.page_tokens, KEYS);
-                        if (gone) seen &= ~((n == 64 ? ~0ull : (1ull << n) - 1ull) << i);
-                    }
-                }
-#pragma unroll
-                for (int tile = 0; tile < TILES; ++tile)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const bool sees = (seen >> (O::first(tile, qd) + i)) & 1ull;
-                        s[tile][i] = sees ? s[tile][i] * a.scale : -INFINITY;
-                    }
-            } else {
-#pragma unroll
-                for (int tile = 0; tile < TILES; ++tile) s[tile] *= a.scale;
-            }
-            float high = s[0][0];
+            const unsigned long long seen = tree_seen<KEYS>(a, w, base, all_there, !there, last_page, low_of[node_of[t] - n0], words_of[node_of[t] - n0]);
 #pragma unroll
             for (int tile = 0; tile < TILES; ++tile)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) high = fmaxf(high, s[tile][i]);
-            high = max_half32(max_row16(high));
-            // The maximum follows the scores only when some row's grows by more than 8 (a factor 2^8): until then the weights are
-            // taken against the older one, and numerator and denominator carry the same factor.
-            if (__ballot(high > m[t] + 8.f) != 0ull) {
-                const float now = fmaxf(m[t], high);
-                const float keep = m[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[t] - now);
-                m[t] = now;
-                l[t] *= keep;
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt) o[t][dt] *= keep;
-            }
-            const float shift = m[t] == -INFINITY ? 0.f : m[t];
-#pragma unroll
-            for (int tile = 0; tile < TILES; ++tile)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s[tile][i] = __builtin_amdgcn_exp2f(s[tile][i] - shift);
-                    l[t] += s[tile][i];                 // (a lane's own keys; the four lanes of a row meet at the end)
-                }
+                for (int i = 0; i < 4; ++i) s[tile][i] = (seen >> (O::first(tile, qd) + i)) & 1ull ? s[tile][i] * a.scale : -INFINITY;
+            tree_softmax<true>(s, m[t], l[t], o[t], 1.f);
             O::values(v, s, o[t]);
-            if (odd_values) {
-                for (int i = 0; i < KEYS; ++i) {
-                    if (!__ballot((seen >> i) & 1ull)) continue;
-                    const int key = base + i;
-                    const T* from = v_pool + __shfl(page, min(key >> a.page_shift, last_page) - first_page, 64) * page_size + head_block +
-                                    (key & page_mask);
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float x = to_float(from[static_cast<size_t>(16 * dt + 4 * qd + e) << a.page_shift]);
-                            if (((seen >> i) & 1ull) && !(fabsf(x) < INFINITY)) o[t][dt][e] += x;
-                        }
-                }
-            }
+            if (odd_values) tree_odd_values<T, KEYS>(o[t], v_pool, page_size, a.page_shift, base, last_page, page, seen);
         }
     }
-    // ---- the four wavefronts' results: the upper two to the lower two, then those
+    // the four wavefronts' results: the upper two to the lower two, then those
 #pragma unroll
     for (int t = 0; t < RT; ++t) l[t] = sum_half32(sum_row16(l[t]));
     for (int half = 2; half >= 1; half >>= 1) {
@@ -374,25 +473,199 @@ __global__ __launch_bounds__(256) void tree_attention_kernel(const TreeArgs a) {
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         const int j = j0 + 16 * t + c;
-        if (j >= rows) continue;
-        const size_t row = first + row_node[t], head = kvh * a.group + j % a.group;
-        if (a.parts == 1) {
-            T* to = static_cast<T*>(a.out) + (row * a.heads + head) * HD + 4 * qd;
-            const float inverse = 1.f / l[t];
+        if (j < w.rows) tree_store<T, HD>(a, w.first + node_of[t], kvh * a.group + j % a.group, part, qd, m[t], l[t], o[t]);
+    }
+}
+
+// ---- many rows, bfloat16: the keys and values of a round are staged in LDS for the four wavefronts, each of which has 16 RT
+// rows of its own.  The next round is fetched into registers while the current one is worked on, and written to the other of two
+// buffers before the one barrier of the round.  Keys lie in LDS in the order of the score tiles, rows 16 bytes longer than they
+// are, so that eight neighbouring lanes read from all banks.
+template <int HD, int RT>
+__global__ __launch_bounds__(256, 2) void tree_rows_kernel(const TreeArgs a) {
+    // (rounds of 64 keys for any head size: staged keys cost no registers)
+    using O = TreeOps<bf16, HD>;
+    using Frag = tree_bf16x8;
+    constexpr int KEYS = 64, TILES = 4, KS = O::KS, DT = O::DT, ROWS = 64 * RT, CH = HD / 8, PER = HD / 32;
+    constexpr int KROW = HD + 8, VROW = KEYS + 8;
+    struct Buffer {
+        __bf16 k[KEYS * KROW];
+        __bf16 v[HD * VROW];
+    };
+    __shared__ __align__(16) Buffer buffers[2];
+    __shared__ int up[TREE_MAX_NODES];
+    __shared__ unsigned long long words_of[ROWS][TREE_MAX_NODES / 64];
+    __shared__ int low_of[ROWS];
+    __shared__ int odd[2];             // the round whose values held infinities or NaN last, plus one
+    const int spread = (a.units + 7) & ~7, block = blockIdx.x / spread, unit = blockIdx.x % spread;
+    if (unit >= a.units) return;
+    const int kvh = unit % a.kv_heads, part = unit / a.kv_heads % a.parts, r = unit / (a.kv_heads * a.parts);
+    const TreeRequest w(a, r);
+    const int b0 = block * ROWS;
+    if (!w.ok || b0 >= w.rows) return;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 15, qd = lane >> 4;
+    const int j0 = b0 + wave * 16 * RT;
+    const bool active = j0 < w.rows;       // (the others only help to stage)
+    const size_t per_head = static_cast<size_t>(HD) << a.page_shift, page_size = per_head * a.kv_heads * a.n_layers;
+    const size_t head_block = per_head * (static_cast<size_t>(a.layer) * a.kv_heads + kvh);
+    const __bf16* __restrict__ k_pool = static_cast<const __bf16*>(a.k_pool) + head_block;
+    const __bf16* __restrict__ v_pool = static_cast<const __bf16*>(a.v_pool) + head_block;
+    const int page_mask = a.page_tokens - 1;
+    Frag q[RT][KS];
+    int node_of[RT];
+    tree_queries<bf16, HD, RT>(a, w, kvh, j0, q, node_of);
+    const int n0 = b0 / a.group, n1 = min(b0 + ROWS - 1, w.rows - 1) / a.group;
+    if (tid < 2) odd[tid] = 0;
+    tree_ways<256>(a, w, n0, n1, up, words_of, low_of);
+    const TreeRounds rounds(a, w, part, KEYS);
+
+    auto top_of = [&](int round) { return min(round * KEYS + KEYS, w.end) - 1; };
+    auto pages_of = [&](int round) {       // the lane's page of a round
+        const int first_page = round * KEYS >> a.page_shift;
+        return w.pages[min(first_page + lane, top_of(round) >> a.page_shift)];
+    };
+    auto is_plain = [&](int round, bool all_there) {
+        return round * KEYS >= rounds.plain && round * KEYS + KEYS <= w.start && all_there;
+    };
+    Frag k_next[PER], v_next[PER];
+    auto fetch = [&](int round, int page) {       // page: valid or 0
+        const int base = round * KEYS, top = top_of(round), first_page = base >> a.page_shift;
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                const float x[4] = {o[t][dt][0] * inverse, o[t][dt][1] * inverse, o[t][dt][2] * inverse, o[t][dt][3] * inverse};
-                Vec4<T>::store(to + 16 * dt, x);
-            }
-        } else {
-            const size_t at = (row * a.heads + head) * a.parts + part;
-            if (qd == 0) {
-                a.ws_ml[2 * at] = m[t];
-                a.ws_ml[2 * at + 1] = l[t];
-            }
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<tree_f4*>(a.ws_o + at * HD + 16 * dt + 4 * qd) = o[t][dt];
+        for (int i = 0; i < PER; ++i) {
+            const int x = tid + 256 * i, key = min(base + x / CH, top);
+            k_next[i] = *reinterpret_cast<const Frag*>(k_pool + __shfl(page, (key >> a.page_shift) - first_page, 64) * page_size +
+                                                       static_cast<size_t>(key & page_mask) * HD + (x % CH) * 8);
         }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            // (pairs of 8 keys by dimensions: a page's values follow one another in memory)
+            const int x = tid + 256 * i, pair = x / (2 * HD), dim = x / 2 % HD, key = min(base + 16 * pair + 8 * (x & 1), top & ~7);
+            v_next[i] = *reinterpret_cast<const Frag*>(v_pool + __shfl(page, (key >> a.page_shift) - first_page, 64) * page_size +
+                                                       (static_cast<size_t>(dim) << a.page_shift) + (key & page_mask));
+        }
+    };
+    auto stage = [&](int round, bool all_there, Buffer& to, int& odd_round) {
+        if (!is_plain(round, all_there)) {
+            unsigned bad = 0;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const unsigned b = O::not_finite(v_next[i]);
+                if (b) O::make_finite(v_next[i]);
+                bad |= b;
+            }
+            if (bad) odd_round = round + 1;
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int x = tid + 256 * i, key = x / CH;
+            const int row = 16 * (2 * (key >> 5) + ((key >> 2) & 1)) + 4 * ((key >> 3) & 3) + (key & 3);
+            *reinterpret_cast<Frag*>(to.k + row * KROW + (x % CH) * 8) = k_next[i];
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int x = tid + 256 * i, pair = x / (2 * HD), dim = x / 2 % HD;
+            *reinterpret_cast<Frag*>(to.v + dim * VROW + 16 * pair + 8 * (x & 1)) = v_next[i];
+        }
+    };
+    float m[RT], l[RT];
+    tree_f4 o[RT][DT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        m[t] = -INFINITY;
+        l[t] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[t][dt] = tree_f4{0.f, 0.f, 0.f, 0.f};
+    }
+    int page = 0, page_after = 0;
+    bool gone = false, all_there = true;
+    if (rounds.r_begin <= rounds.r_end) {
+        page = pages_of(rounds.r_begin);
+        gone = page < 0 || page >= a.n_pages;
+        all_there = __ballot(gone) == 0ull;
+        page = gone ? 0 : page;
+        fetch(rounds.r_begin, page);
+        if (rounds.r_begin < rounds.r_end) page_after = pages_of(rounds.r_begin + 1);
+        stage(rounds.r_begin, all_there, buffers[0], odd[0]);
+    }
+    int cur = 0;
+    for (int round = rounds.r_begin; round <= rounds.r_end; ++round, cur ^= 1) {
+        __syncthreads();
+        const bool more = round < rounds.r_end;
+        bool gone_next = false, there_next = true;
+        int page_next = 0;
+        if (more) {
+            page_next = page_after;
+            gone_next = page_next < 0 || page_next >= a.n_pages;
+            there_next = __ballot(gone_next) == 0ull;
+            page_next = gone_next ? 0 : page_next;
+            fetch(round + 1, page_next);
+            if (round + 1 < rounds.r_end) page_after = pages_of(round + 2);
+        }
+        const Buffer& from = buffers[cur];
+        if (active) {
+            const int base = round * KEYS;
+            tree_f4 s[RT][TILES];
+#pragma unroll
+            for (int tile = 0; tile < TILES; ++tile) {
+                Frag k[KS];
+#pragma unroll
+                for (int x = 0; x < KS; ++x) k[x] = *reinterpret_cast<const Frag*>(from.k + (16 * tile + c) * KROW + 32 * x + 8 * qd);
+#pragma unroll
+                for (int t = 0; t < RT; ++t) s[t][tile] = O::scores(k, q[t]);
+            }
+            const bool plain = is_plain(round, all_there);
+            unsigned long long seen[RT];
+            if (plain) {
+#pragma unroll
+                for (int t = 0; t < RT; ++t) tree_softmax<false>(s[t], m[t], l[t], o[t], a.scale);
+            } else {
+#pragma unroll
+                for (int t = 0; t < RT; ++t) {
+                    seen[t] = tree_seen<KEYS>(a, w, base, all_there, gone, top_of(round) >> a.page_shift, low_of[node_of[t] - n0],
+                                              words_of[node_of[t] - n0]);
+#pragma unroll
+                    for (int tile = 0; tile < TILES; ++tile)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            s[t][tile][i] = (seen[t] >> (32 * (tile >> 1) + 8 * qd + 4 * (tile & 1) + i)) & 1ull ? s[t][tile][i] * a.scale : -INFINITY;
+                    tree_softmax<true>(s[t], m[t], l[t], o[t], 1.f);
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                Frag p[RT];
+#pragma unroll
+                for (int t = 0; t < RT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        p[t][i] = static_cast<__bf16>(s[t][2 * g][i]);
+                        p[t][4 + i] = static_cast<__bf16>(s[t][2 * g + 1][i]);
+                    }
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    const Frag v = *reinterpret_cast<const Frag*>(from.v + (16 * dt + c) * VROW + 32 * g + 8 * qd);
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[t], o[t][dt], 0, 0, 0);
+                }
+            }
+            if (!plain && odd[cur] == round + 1) {
+#pragma unroll
+                for (int t = 0; t < RT; ++t)
+                    tree_odd_values<bf16, KEYS>(o[t], reinterpret_cast<const bf16*>(v_pool), page_size, a.page_shift, base,
+                                                top_of(round) >> a.page_shift, page, seen[t]);
+            }
+        }
+        if (more) stage(round + 1, there_next, buffers[cur ^ 1], odd[cur ^ 1]);
+        page = page_next;
+        gone = gone_next;
+        all_there = there_next;
+    }
+    if (!active) return;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        l[t] = sum_half32(sum_row16(l[t]));
+        const int j = j0 + 16 * t + c;
+        if (j < w.rows) tree_store<bf16, HD>(a, w.first + node_of[t], kvh * a.group + j % a.group, part, qd, m[t], l[t], o[t]);
     }
 }
 
@@ -426,12 +699,16 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeArgs a) {
         if (lane + 64 * e < HD) to[lane + 64 * e] = from_float<T>(o[e] / sum);
 }
 
-// Rows a workgroup takes (16 times this) and keys of a round, for these sizes.
-static int tree_row_tiles(int dtype, int head_dim, int rows) {
-    const int most = dtype == CELEG_BF16 ? (head_dim <= 64 ? 4 : 2) : (head_dim <= 64 ? 2 : 1);
-    return rows <= 16 ? 1 : rows <= 32 || most == 2 ? std::min(2, most) : most;
+// The form of a launch: rows of a workgroup, and keys of a round.
+struct TreeForm {
+    bool staged;
+    int tiles, rows, keys;
+};
+static TreeForm tree_form(int dtype, int head_dim, int rows) {
+    if (dtype == CELEG_BF16 && rows > 32) return rows <= 64 ? TreeForm{true, 1, 64, 64} : TreeForm{true, 2, 128, 64};
+    const int tiles = rows <= 16 || (dtype != CELEG_BF16 && head_dim > 64) ? 1 : 2;
+    return {false, tiles, 16 * tiles, dtype == CELEG_BF16 && head_dim <= 64 ? 64 : 32};
 }
-static int tree_round_keys(int dtype, int head_dim) { return dtype == CELEG_BF16 && head_dim <= 64 ? 64 : 32; }
 
 // Whether the matrix cores take these sizes.
 extern "C" int celeg_tree_attention_fast_ok(int head_dim, int page_tokens) {
@@ -440,10 +717,11 @@ extern "C" int celeg_tree_attention_fast_ok(int head_dim, int page_tokens) {
 
 // Parts that the contexts are cut into: about two workgroups a compute unit, each wavefront with a round at least.
 extern "C" int celeg_tree_attention_parts(int dtype, int head_dim, int requests, int kv_heads, int group, int max_nodes, int max_context) {
-    const int rows = max_nodes * group, block = 16 * tree_row_tiles(dtype, head_dim, rows), keys = tree_round_keys(dtype, head_dim);
-    const long long groups = static_cast<long long>(requests) * kv_heads * ((rows + block - 1) / block);
-    const long long rounds = (static_cast<long long>(max_context) + max_nodes + keys - 1) / keys;
-    return static_cast<int>(std::max(1LL, std::min({(512 + groups - 1) / groups, (rounds + 3) / 4, 64LL})));
+    const int rows = max_nodes * group;
+    const TreeForm form = tree_form(dtype, head_dim, rows);
+    const long long groups = static_cast<long long>(requests) * kv_heads * ((rows + form.rows - 1) / form.rows);
+    const long long rounds = (static_cast<long long>(max_context) + max_nodes + form.keys - 1) / form.keys;
+    return static_cast<int>(std::max(1LL, std::min({(512 + groups - 1) / groups, form.staged ? (rounds + 1) / 2 : (rounds + 3) / 4, 64LL})));
 }
 
 extern "C" int celeg_tree_attention_fast(const void* q, int ldq, int dtype, const void* k_pool, const void* v_pool, int n_pages, int n_layers,
@@ -479,23 +757,28 @@ extern "C" int celeg_tree_attention_fast(const void* q, int ldq, int dtype, cons
     a.max_nodes = max_nodes;
     a.parts = parts;
     a.units = n_requests * kv_heads * parts;
-    a.scale = scale * 1.44269504088896340736f;
+    a.scale = fabsf(scale) * 1.44269504088896340736f;
+    a.turned = scale < 0.f;
     a.window = window;
-    const int rows = max_nodes * a.group, tiles = tree_row_tiles(dtype, head_dim, rows);
-    a.row_blocks = (rows + 16 * tiles - 1) / (16 * tiles);
+    const int rows = max_nodes * a.group;
+    const TreeForm form = tree_form(dtype, head_dim, rows);
+    a.row_blocks = (rows + form.rows - 1) / form.rows;
     const dim3 grid(static_cast<unsigned>((a.units + 7) / 8 * 8) * a.row_blocks);
     const dim3 join(static_cast<unsigned>((static_cast<long long>(n_requests) * max_nodes * heads + 3) / 4));
     auto run = [&](auto* type, auto dim) {
         using T = std::remove_pointer_t<decltype(type)>;
         constexpr int HD = decltype(dim)::value;
         constexpr bool B = std::is_same<T, bf16>::value;
-        if constexpr ((B && HD <= 64)) {
-            if (tiles == 4) tree_attention_kernel<T, HD, 4><<<grid, dim3(256), 0, stream>>>(a);
+        if (form.staged) {
+            if constexpr (B) {
+                if (form.tiles == 2) tree_rows_kernel<HD, 2><<<grid, dim3(256), 0, stream>>>(a);
+                else tree_rows_kernel<HD, 1><<<grid, dim3(256), 0, stream>>>(a);
+            }
+        } else if (form.tiles == 2) {
+            if constexpr (B || HD <= 64) tree_few_kernel<T, HD, 2><<<grid, dim3(256), 0, stream>>>(a);
+        } else {
+            tree_few_kernel<T, HD, 1><<<grid, dim3(256), 0, stream>>>(a);
         }
-        if constexpr (B || HD <= 64) {
-            if (tiles == 2) tree_attention_kernel<T, HD, 2><<<grid, dim3(256), 0, stream>>>(a);
-        }
-        if (tiles == 1) tree_attention_kernel<T, HD, 1><<<grid, dim3(256), 0, stream>>>(a);
         if (parts > 1) tree_join_kernel<T, HD><<<join, dim3(256), 0, stream>>>(a);
     };
     auto by_dim = [&](auto* type) {
