@@ -46,15 +46,19 @@ struct TreeArgs {
 };
 
 // How keys and values lie in the operands.  A round holds KEYS keys; `a` of a key tile is 16 keys by the head's values, a
-// lane's (c, qd) = (lane % 16, lane / 16) share of it key KEY(tile, c); a score tile leaves a lane the scores of row c with the four
-// keys FIRST(tile, qd) .. + 3 of the round, which are in turn the keys that it has to hold of the values.
+// lane's (c, qd) = (lane % 16, lane / 16) share of it key(tile, c); a score tile leaves a lane the scores of row c with four keys that
+// follow one another, which are in turn the keys that the lane's weights have to stand for in the product with the values.
 template <typename T, int HD> struct TreeOps;
 
 template <int HD> struct TreeOps<bf16, HD> {
     static constexpr int KEYS = HD <= 64 ? 64 : 32, TILES = KEYS / 16, KS = HD / 32, DT = HD / 16, VG = KEYS / 32, VKEYS = 8;
     typedef tree_bf16x8 Frag;
     static __device__ __forceinline__ int key(int tile, int c) { return 32 * (tile >> 1) + 8 * (c >> 2) + 4 * (tile & 1) + (c & 3); }
-    static __device__ __forceinline__ int first(int tile, int qd) { return 32 * (tile >> 1) + 8 * qd + 4 * (tile & 1); }
+    // whether a row that sees the keys of `seen` sees those of its scores: bits of the word that shown() gives
+    static __device__ __forceinline__ unsigned shown(unsigned long long seen, int tile, int qd) {
+        return static_cast<unsigned>(tile >> 1 ? seen >> 32 : seen) >> (8 * qd);
+    }
+    static __device__ __forceinline__ constexpr int bit(int tile, int i) { return 4 * (tile & 1) + i; }
     static __device__ __forceinline__ int vkey(int g, int qd) { return 32 * g + 8 * qd; }
     static __device__ __forceinline__ int dim(int s, int qd) { return 32 * s + 8 * qd; }
     static __device__ __forceinline__ tree_f4 scores(const Frag (&k)[KS], const Frag (&q)[KS]) {
@@ -99,7 +103,8 @@ template <int HD> struct TreeOps<float, HD> {
     static constexpr int KEYS = 32, TILES = KEYS / 16, KS = HD / 16, DT = HD / 16, VG = TILES, VKEYS = 4;
     typedef tree_f4 Frag;
     static __device__ __forceinline__ int key(int tile, int c) { return 16 * tile + c; }
-    static __device__ __forceinline__ int first(int tile, int qd) { return 16 * tile + 4 * qd; }
+    static __device__ __forceinline__ unsigned shown(unsigned long long seen, int, int qd) { return static_cast<unsigned>(seen) >> (4 * qd); }
+    static __device__ __forceinline__ constexpr int bit(int tile, int i) { return 16 * tile + i; }
     static __device__ __forceinline__ int vkey(int g, int qd) { return 16 * g + 4 * qd; }
     // (a product sums over the head's values in any order: a lane holds a quarter of them that lie side by side)
     static __device__ __forceinline__ int dim(int s, int qd) { return (HD / 4) * qd + 4 * s; }
@@ -160,10 +165,11 @@ struct TreeRequest {
     bool ok;
     const int* pages;
     __device__ __forceinline__ TreeRequest(const TreeArgs& a, int r) {
-        first = a.offsets[r];
-        count = min(min(a.offsets[r + 1], a.n_rows) - first, a.max_nodes);
-        slot = a.slots[r];
-        start = max(a.starts[r], 0);
+        // (the same for all lanes: said so that they take no vector registers)
+        first = __builtin_amdgcn_readfirstlane(a.offsets[r]);
+        count = __builtin_amdgcn_readfirstlane(min(min(a.offsets[r + 1], a.n_rows) - first, a.max_nodes));
+        slot = __builtin_amdgcn_readfirstlane(a.slots[r]);
+        start = __builtin_amdgcn_readfirstlane(max(a.starts[r], 0));
         rows = count * a.group;
         // (places behind what the table holds are seen by nobody)
         const int room = a.table_stride << a.page_shift;
@@ -340,7 +346,7 @@ __device__ __forceinline__ void tree_queries(const TreeArgs& a, const TreeReques
 
 // ---- few rows: operands straight from memory, the wavefronts take the rounds in turn
 template <typename T, int HD, int RT>
-__global__ __launch_bounds__(256) void tree_few_kernel(const TreeArgs a) {
+__global__ __launch_bounds__(256, 2) void tree_few_kernel(const TreeArgs a) {
     using O = TreeOps<T, HD>;
     using Frag = typename O::Frag;
     constexpr int KEYS = O::KEYS, TILES = O::TILES, KS = O::KS, DT = O::DT, VG = O::VG, ROWS = 16 * RT;
@@ -433,7 +439,8 @@ __global__ __launch_bounds__(256) void tree_few_kernel(const TreeArgs a) {
 #pragma unroll
             for (int tile = 0; tile < TILES; ++tile)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[tile][i] = (seen >> (O::first(tile, qd) + i)) & 1ull ? s[tile][i] * a.scale : -INFINITY;
+                for (int i = 0; i < 4; ++i)
+                    s[tile][i] = (O::shown(seen, tile, qd) >> O::bit(tile, i)) & 1u ? s[tile][i] * a.scale : -INFINITY;
             tree_softmax<true>(s, m[t], l[t], o[t], 1.f);
             O::values(v, s, o[t]);
             if (odd_values) tree_odd_values<T, KEYS>(o[t], v_pool, page_size, a.page_shift, base, last_page, page, seen);
@@ -478,25 +485,26 @@ __global__ __launch_bounds__(256) void tree_few_kernel(const TreeArgs a) {
 }
 
 // ---- many rows, bfloat16: the keys and values of a round are staged in LDS for the four wavefronts, each of which has 16 RT
-// rows of its own.  The next round is fetched into registers while the current one is worked on, and written to the other of two
-// buffers before the one barrier of the round.  Keys lie in LDS in the order of the score tiles, rows 16 bytes longer than they
-// are, so that eight neighbouring lanes read from all banks.
+// rows of its own.  The next round travels straight from memory to the other of two buffers while the current one is worked on.
+// Keys lie in LDS in the order of the score tiles; the 16-byte pieces of a row change places by the row's number, so that eight
+// neighbouring lanes, which read the same piece of as many rows, read from all banks.
+#define TREE_GLOBAL(p) reinterpret_cast<const __attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(p))
+#define TREE_LDS(p) reinterpret_cast<__attribute__((address_space(3))) void*>(reinterpret_cast<uintptr_t>(p))
+
 template <int HD, int RT>
 __global__ __launch_bounds__(256, 2) void tree_rows_kernel(const TreeArgs a) {
     // (rounds of 64 keys for any head size: staged keys cost no registers)
     using O = TreeOps<bf16, HD>;
     using Frag = tree_bf16x8;
     constexpr int KEYS = 64, TILES = 4, KS = O::KS, DT = O::DT, ROWS = 64 * RT, CH = HD / 8, PER = HD / 32;
-    constexpr int KROW = HD + 8, VROW = KEYS + 8;
     struct Buffer {
-        __bf16 k[KEYS * KROW];
-        __bf16 v[HD * VROW];
+        __bf16 k[KEYS * HD];
+        __bf16 v[HD * KEYS];
     };
-    __shared__ __align__(16) Buffer buffers[2];
+    __shared__ __align__(1024) Buffer buffers[2];
     __shared__ int up[TREE_MAX_NODES];
     __shared__ unsigned long long words_of[ROWS][TREE_MAX_NODES / 64];
     __shared__ int low_of[ROWS];
-    __shared__ int odd[2];             // the round whose values held infinities or NaN last, plus one
     const int spread = (a.units + 7) & ~7, block = blockIdx.x / spread, unit = blockIdx.x % spread;
     if (unit >= a.units) return;
     const int kvh = unit % a.kv_heads, part = unit / a.kv_heads % a.parts, r = unit / (a.kv_heads * a.parts);
@@ -515,7 +523,6 @@ __global__ __launch_bounds__(256, 2) void tree_rows_kernel(const TreeArgs a) {
     int node_of[RT];
     tree_queries<bf16, HD, RT>(a, w, kvh, j0, q, node_of);
     const int n0 = b0 / a.group, n1 = min(b0 + ROWS - 1, w.rows - 1) / a.group;
-    if (tid < 2) odd[tid] = 0;
     tree_ways<256>(a, w, n0, n1, up, words_of, low_of);
     const TreeRounds rounds(a, w, part, KEYS);
 
@@ -524,49 +531,44 @@ __global__ __launch_bounds__(256, 2) void tree_rows_kernel(const TreeArgs a) {
         const int first_page = round * KEYS >> a.page_shift;
         return w.pages[min(first_page + lane, top_of(round) >> a.page_shift)];
     };
-    auto is_plain = [&](int round, bool all_there) {
-        return round * KEYS >= rounds.plain && round * KEYS + KEYS <= w.start && all_there;
-    };
-    Frag k_next[PER], v_next[PER];
-    auto fetch = [&](int round, int page) {       // page: valid or 0
+    // A wavefront's i-th instruction fills 64 pieces of 16 bytes from piece 64 (wave + 4 i) of the keys (values) on: the lane's row of
+    // keys is CH pieces long, and of values 8.  The pieces are numbered so that what hangs on the lane is the same for every i.
+    constexpr bool EVEN = HD % 64 == 0;
+    const int v_dim = 8 * wave + (lane >> 3), v_key = 8 * ((lane & 7) ^ ((lane >> 3) & 7));      // dimension v_dim + 32 i
+    const int k_row = 64 * wave / CH + lane / CH;                                                  // row k_row + 256 i / CH, if EVEN
+    const int k_piece = HD == 32 ? (lane & 3) ^ ((k_row >> 1) & 3) : (lane % CH) ^ (k_row & 7);
+    auto key_of_row = [](int row) { return 32 * (row >> 5) + 8 * ((row >> 2) & 3) + 4 * ((row >> 4) & 1) + (row & 3); };
+    auto fetch = [&](int round, int page, Buffer& to) {       // page: valid or 0
         const int base = round * KEYS, top = top_of(round), first_page = base >> a.page_shift;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int x = tid + 256 * i, key = min(base + x / CH, top);
-            k_next[i] = *reinterpret_cast<const Frag*>(k_pool + __shfl(page, (key >> a.page_shift) - first_page, 64) * page_size +
-                                                       static_cast<size_t>(key & page_mask) * HD + (x % CH) * 8);
-        }
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            // (pairs of 8 keys by dimensions: a page's values follow one another in memory)
-            const int x = tid + 256 * i, pair = x / (2 * HD), dim = x / 2 % HD, key = min(base + 16 * pair + 8 * (x & 1), top & ~7);
-            v_next[i] = *reinterpret_cast<const Frag*>(v_pool + __shfl(page, (key >> a.page_shift) - first_page, 64) * page_size +
-                                                       (static_cast<size_t>(dim) << a.page_shift) + (key & page_mask));
-        }
-    };
-    auto stage = [&](int round, bool all_there, Buffer& to, int& odd_round) {
-        if (!is_plain(round, all_there)) {
-            unsigned bad = 0;
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const unsigned b = O::not_finite(v_next[i]);
-                if (b) O::make_finite(v_next[i]);
-                bad |= b;
+            int row_key, piece;
+            if (EVEN || PER == 1) {
+                // (rows 16 apart at 128 values: tiles of 4 keys further on, or 32; rows 32 apart at 64: 32)
+                row_key = key_of_row(k_row) + (HD == 128 ? 32 * (i >> 1) + 4 * (i & 1) : 32 * i);
+                piece = k_piece;
+            } else {
+                const int x = (wave + 4 * i) * 64 + lane, row = x / CH;
+                row_key = key_of_row(row);
+                piece = (x % CH) ^ (row & 3);
             }
-            if (bad) odd_round = round + 1;
+            const int key = min(base + row_key, top);
+            const __bf16* from = k_pool + __shfl(page, (key >> a.page_shift) - first_page, 64) * page_size +
+                                 (static_cast<size_t>(key & page_mask) * HD + piece * 8);
+            __builtin_amdgcn_global_load_lds(TREE_GLOBAL(from), TREE_LDS(to.k + (wave + 4 * i) * 512), 16, 0, 0);
         }
+        const int key = min(base + v_key, top & ~7);
+        const __bf16* from = v_pool + __shfl(page, (key >> a.page_shift) - first_page, 64) * page_size +
+                             ((static_cast<size_t>(v_dim) << a.page_shift) + (key & page_mask));
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int x = tid + 256 * i, key = x / CH;
-            const int row = 16 * (2 * (key >> 5) + ((key >> 2) & 1)) + 4 * ((key >> 3) & 3) + (key & 3);
-            *reinterpret_cast<Frag*>(to.k + row * KROW + (x % CH) * 8) = k_next[i];
-        }
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int x = tid + 256 * i, pair = x / (2 * HD), dim = x / 2 % HD;
-            *reinterpret_cast<Frag*>(to.v + dim * VROW + 16 * pair + 8 * (x & 1)) = v_next[i];
-        }
+        for (int i = 0; i < PER; ++i)
+            __builtin_amdgcn_global_load_lds(TREE_GLOBAL(from + (static_cast<size_t>(32 * i) << a.page_shift)),
+                                             TREE_LDS(to.v + (wave + 4 * i) * 512), 16, 0, 0);
     };
+    // where the lane's pieces of a row lie in LDS
+    const int piece0 = EVEN ? qd ^ (c & 7) : HD == 96 ? qd ^ (c & 3) : qd ^ ((c >> 1) & 3), piece1 = (4 + qd) ^ (c & 7);
+    const int v_piece0 = qd ^ (c & 7);
+    auto k_piece_of = [&](int x) { return EVEN ? (x & 1 ? piece1 : piece0) + 8 * (x >> 1) : piece0 + 4 * x; };
     float m[RT], l[RT];
     tree_f4 o[RT][DT];
 #pragma unroll
@@ -583,79 +585,104 @@ __global__ __launch_bounds__(256, 2) void tree_rows_kernel(const TreeArgs a) {
         gone = page < 0 || page >= a.n_pages;
         all_there = __ballot(gone) == 0ull;
         page = gone ? 0 : page;
-        fetch(rounds.r_begin, page);
+        fetch(rounds.r_begin, page, buffers[0]);
         if (rounds.r_begin < rounds.r_end) page_after = pages_of(rounds.r_begin + 1);
-        stage(rounds.r_begin, all_there, buffers[0], odd[0]);
     }
     int cur = 0;
     for (int round = rounds.r_begin; round <= rounds.r_end; ++round, cur ^= 1) {
-        __syncthreads();
-        const bool more = round < rounds.r_end;
+        // the round has arrived, for all wavefronts, and nobody reads the other buffer any more
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
         bool gone_next = false, there_next = true;
         int page_next = 0;
-        if (more) {
+        if (round < rounds.r_end) {
             page_next = page_after;
             gone_next = page_next < 0 || page_next >= a.n_pages;
             there_next = __ballot(gone_next) == 0ull;
             page_next = gone_next ? 0 : page_next;
-            fetch(round + 1, page_next);
+            fetch(round + 1, page_next, buffers[cur ^ 1]);
             if (round + 1 < rounds.r_end) page_after = pages_of(round + 2);
         }
         const Buffer& from = buffers[cur];
-        if (active) {
-            const int base = round * KEYS;
+        auto keys_of = [&](int tile, int x) {
+            return *reinterpret_cast<const Frag*>(from.k + (16 * tile + c) * HD + k_piece_of(x) * 8);
+        };
+        auto values_of = [&](int dt, int g) {
+            return *reinterpret_cast<const Frag*>(from.v + (16 * dt + c) * KEYS + (g ? piece1 : v_piece0) * 8);
+        };
+        auto weights_of = [&](const tree_f4 (&s)[TILES], int g) {
+            Frag p;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p[i] = static_cast<__bf16>(s[2 * g][i]);
+                p[4 + i] = static_cast<__bf16>(s[2 * g + 1][i]);
+            }
+            return p;
+        };
+        const int base = round * KEYS;
+        if (active && base >= rounds.plain && base + KEYS <= w.start && all_there) {
             tree_f4 s[RT][TILES];
 #pragma unroll
             for (int tile = 0; tile < TILES; ++tile) {
                 Frag k[KS];
 #pragma unroll
-                for (int x = 0; x < KS; ++x) k[x] = *reinterpret_cast<const Frag*>(from.k + (16 * tile + c) * KROW + 32 * x + 8 * qd);
+                for (int x = 0; x < KS; ++x) k[x] = keys_of(tile, x);
 #pragma unroll
                 for (int t = 0; t < RT; ++t) s[t][tile] = O::scores(k, q[t]);
             }
-            const bool plain = is_plain(round, all_there);
-            unsigned long long seen[RT];
-            if (plain) {
 #pragma unroll
-                for (int t = 0; t < RT; ++t) tree_softmax<false>(s[t], m[t], l[t], o[t], a.scale);
-            } else {
-#pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    seen[t] = tree_seen<KEYS>(a, w, base, all_there, gone, top_of(round) >> a.page_shift, low_of[node_of[t] - n0],
-                                              words_of[node_of[t] - n0]);
-#pragma unroll
-                    for (int tile = 0; tile < TILES; ++tile)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            s[t][tile][i] = (seen[t] >> (32 * (tile >> 1) + 8 * qd + 4 * (tile & 1) + i)) & 1ull ? s[t][tile][i] * a.scale : -INFINITY;
-                    tree_softmax<true>(s[t], m[t], l[t], o[t], 1.f);
-                }
-            }
+            for (int t = 0; t < RT; ++t) tree_softmax<false>(s[t], m[t], l[t], o[t], a.scale);
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 Frag p[RT];
 #pragma unroll
-                for (int t = 0; t < RT; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        p[t][i] = static_cast<__bf16>(s[t][2 * g][i]);
-                        p[t][4 + i] = static_cast<__bf16>(s[t][2 * g + 1][i]);
-                    }
+                for (int t = 0; t < RT; ++t) p[t] = weights_of(s[t], g);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
-                    const Frag v = *reinterpret_cast<const Frag*>(from.v + (16 * dt + c) * VROW + 32 * g + 8 * qd);
+                    const Frag v = values_of(dt, g);
 #pragma unroll
                     for (int t = 0; t < RT; ++t) o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[t], o[t][dt], 0, 0, 0);
                 }
             }
-            if (!plain && odd[cur] == round + 1) {
+        } else if (active) {
+            // A weight of 0 times an infinity or a NaN is no 0: such values are taken out, and added for the rows that see them
+            const int last_page = top_of(round) >> a.page_shift;
 #pragma unroll
-                for (int t = 0; t < RT; ++t)
-                    tree_odd_values<bf16, KEYS>(o[t], reinterpret_cast<const bf16*>(v_pool), page_size, a.page_shift, base,
-                                                top_of(round) >> a.page_shift, page, seen[t]);
+            for (int t = 0; t < RT; ++t) {
+                tree_f4 s[TILES];
+#pragma unroll
+                for (int tile = 0; tile < TILES; ++tile) {
+                    Frag k[KS];
+#pragma unroll
+                    for (int x = 0; x < KS; ++x) k[x] = keys_of(tile, x);
+                    s[tile] = O::scores(k, q[t]);
+                }
+                const unsigned long long seen = tree_seen<KEYS>(a, w, base, all_there, gone, last_page, low_of[node_of[t] - n0], words_of[node_of[t] - n0]);
+                const unsigned mine[2] = {static_cast<unsigned>(seen) >> (8 * qd), static_cast<unsigned>(seen >> 32) >> (8 * qd)};
+#pragma unroll
+                for (int tile = 0; tile < TILES; ++tile)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        s[tile][i] = (mine[tile >> 1] >> (4 * (tile & 1) + i)) & 1u ? s[tile][i] * a.scale : -INFINITY;
+                tree_softmax<true>(s, m[t], l[t], o[t], 1.f);
+                unsigned bad = 0;
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    const Frag p = weights_of(s, g);
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) {
+                        Frag v = values_of(dt, g);
+                        const unsigned b = O::not_finite(v);
+                        if (b) O::make_finite(v);
+                        bad |= b;
+                        o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p, o[t][dt], 0, 0, 0);
+                    }
+                }
+                if (__ballot(bad != 0))
+                    tree_odd_values<bf16, KEYS>(o[t], reinterpret_cast<const bf16*>(v_pool), page_size, a.page_shift, base, last_page, page, seen);
             }
         }
-        if (more) stage(round + 1, there_next, buffers[cur ^ 1], odd[cur ^ 1]);
         page = page_next;
         gone = gone_next;
         all_there = there_next;
