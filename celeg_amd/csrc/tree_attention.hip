@@ -220,37 +220,49 @@ struct TreeRounds {
     }
 };
 
-// One row tile's scores of a round into weights, its running maximum m (in powers of two), sum l (a lane's own keys; the four
-// lanes of a row meet at the end) and output o brought up to date.  MASKED: the scores are scaled and hidden ones -inf already.
-// The maximum follows the scores only when some row's grows by more than 8 (a factor 2^8): until then the weights are taken against the
-// older one, and numerator and denominator carry the same factor.
-template <bool MASKED, int TILES, int DT>
-__device__ __forceinline__ void tree_softmax(tree_f4 (&s)[TILES], float& m, float& l, tree_f4 (&o)[DT], float scale) {
-    float high = s[0][0];
+// The scores of a round, of RT row tiles, into weights; the rows' running maximum m (in powers of two), sum l (a lane's own keys;
+// the four lanes of a row meet at the end) and output o brought up to date.  MASKED: the scores are scaled and hidden ones -inf
+// already.  The maximum follows the scores only when some row's grows by more than 8 (a factor 2^8): until then the weights are taken
+// against the older one, and numerator and denominator carry the same factor.  Whether one grows so far needs no exchange between the
+// lanes of a row: one of them sees it.
+template <bool MASKED, int RT, int TILES, int DT>
+__device__ __forceinline__ void tree_softmax(tree_f4 (&s)[RT][TILES], float (&m)[RT], float (&l)[RT], tree_f4 (&o)[RT][DT], float scale) {
+    float high[RT];
+    bool grows = false;
 #pragma unroll
-    for (int tile = 0; tile < TILES; ++tile)
+    for (int t = 0; t < RT; ++t) {
+        high[t] = s[t][0][0];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) high = fmaxf(high, s[tile][i]);
-    high = max_half32(max_row16(high));
-    if (!MASKED) high *= scale;
-    if (__ballot(high > m + 8.f) != 0ull) {
-        const float now = fmaxf(m, high);
-        const float keep = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - now);
-        m = now;
-        l *= keep;
+        for (int tile = 0; tile < TILES; ++tile)
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[dt] *= keep;
+            for (int i = 0; i < 4; ++i) high[t] = fmaxf(high[t], s[t][tile][i]);
+        if (!MASKED) high[t] *= scale;
+        grows |= high[t] > m[t] + 8.f;
     }
-    const float shift = m == -INFINITY ? 0.f : m;
-    float sum = 0.f;
+    if (__ballot(grows) != 0ull) {
 #pragma unroll
-    for (int tile = 0; tile < TILES; ++tile)
+        for (int t = 0; t < RT; ++t) {
+            const float now = fmaxf(m[t], max_half32(max_row16(high[t])));
+            const float keep = m[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[t] - now);
+            m[t] = now;
+            l[t] *= keep;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            s[tile][i] = __builtin_amdgcn_exp2f(MASKED ? s[tile][i] - shift : fmaf(s[tile][i], scale, -shift));
-            sum += s[tile][i];
+            for (int dt = 0; dt < DT; ++dt) o[t][dt] *= keep;
         }
-    l += sum;
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const float shift = m[t] == -INFINITY ? 0.f : m[t];
+        tree_f4 sum = tree_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int tile = 0; tile < TILES; ++tile) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                s[t][tile][i] = __builtin_amdgcn_exp2f(MASKED ? s[t][tile][i] - shift : fmaf(s[t][tile][i], scale, -shift));
+            sum += s[t][tile];
+        }
+        l[t] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    }
 }
 
 // The keys of the round from `base` on that a row sees, a bit each (page: the lane's page of the round, `gone` if it is none).
@@ -407,14 +419,14 @@ __global__ __launch_bounds__(256, 2) void tree_few_kernel(const TreeArgs a) {
                 v[dt][g] = *reinterpret_cast<const Frag*>(from + (static_cast<size_t>(16 * dt + c) << a.page_shift));
         }
         if (base >= rounds.plain && base + KEYS <= w.start && all_there) {
+            tree_f4 s[RT][TILES];
 #pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                tree_f4 s[TILES];
+            for (int t = 0; t < RT; ++t)
 #pragma unroll
-                for (int tile = 0; tile < TILES; ++tile) s[tile] = O::scores(k[tile], q[t]);
-                tree_softmax<false>(s, m[t], l[t], o[t], a.scale);
-                O::values(v, s, o[t]);
-            }
+                for (int tile = 0; tile < TILES; ++tile) s[t][tile] = O::scores(k[tile], q[t]);
+            tree_softmax<false>(s, m, l, o, a.scale);
+#pragma unroll
+            for (int t = 0; t < RT; ++t) O::values(v, s[t], o[t]);
             continue;
         }
         // A weight of 0 times an infinity or a NaN is no 0: such values are taken out, and added for the rows that see them
@@ -430,20 +442,25 @@ __global__ __launch_bounds__(256, 2) void tree_few_kernel(const TreeArgs a) {
 #pragma unroll
                 for (int g = 0; g < VG; ++g) O::make_finite(v[dt][g]);
         }
+        tree_f4 s[RT][TILES];
+        unsigned long long seen_of[RT];
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-            tree_f4 s[TILES];
 #pragma unroll
-            for (int tile = 0; tile < TILES; ++tile) s[tile] = O::scores(k[tile], q[t]);
+            for (int tile = 0; tile < TILES; ++tile) s[t][tile] = O::scores(k[tile], q[t]);
             const unsigned long long seen = tree_seen<KEYS>(a, w, base, all_there, !there, last_page, low_of[node_of[t] - n0], words_of[node_of[t] - n0]);
 #pragma unroll
             for (int tile = 0; tile < TILES; ++tile)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    s[tile][i] = (O::shown(seen, tile, qd) >> O::bit(tile, i)) & 1u ? s[tile][i] * a.scale : -INFINITY;
-            tree_softmax<true>(s, m[t], l[t], o[t], 1.f);
-            O::values(v, s, o[t]);
-            if (odd_values) tree_odd_values<T, KEYS>(o[t], v_pool, page_size, a.page_shift, base, last_page, page, seen);
+                    s[t][tile][i] = (O::shown(seen, tile, qd) >> O::bit(tile, i)) & 1u ? s[t][tile][i] * a.scale : -INFINITY;
+            seen_of[t] = seen;
+        }
+        tree_softmax<true>(s, m, l, o, 1.f);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            O::values(v, s[t], o[t]);
+            if (odd_values) tree_odd_values<T, KEYS>(o[t], v_pool, page_size, a.page_shift, base, last_page, page, seen_of[t]);
         }
     }
     // the four wavefronts' results: the upper two to the lower two, then those
@@ -495,6 +512,7 @@ template <int HD, int RT>
 __global__ __launch_bounds__(256, 2) void tree_rows_kernel(const TreeArgs a) {
     // (rounds of 64 keys for any head size: staged keys cost no registers)
     using O = TreeOps<bf16, HD>;
+    using O64 = TreeOps<bf16, 64>;
     using Frag = tree_bf16x8;
     constexpr int KEYS = 64, TILES = 4, KS = O::KS, DT = O::DT, ROWS = 64 * RT, CH = HD / 8, PER = HD / 32;
     struct Buffer {
@@ -631,8 +649,7 @@ __global__ __launch_bounds__(256, 2) void tree_rows_kernel(const TreeArgs a) {
 #pragma unroll
                 for (int t = 0; t < RT; ++t) s[t][tile] = O::scores(k, q[t]);
             }
-#pragma unroll
-            for (int t = 0; t < RT; ++t) tree_softmax<false>(s[t], m[t], l[t], o[t], a.scale);
+            tree_softmax<false>(s, m, l, o, a.scale);
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 Frag p[RT];
@@ -648,39 +665,46 @@ __global__ __launch_bounds__(256, 2) void tree_rows_kernel(const TreeArgs a) {
         } else if (active) {
             // A weight of 0 times an infinity or a NaN is no 0: such values are taken out, and added for the rows that see them
             const int last_page = top_of(round) >> a.page_shift;
+            tree_f4 s[RT][TILES];
+            unsigned long long seen[RT];
+#pragma unroll
+            for (int tile = 0; tile < TILES; ++tile) {
+                Frag k[KS];
+#pragma unroll
+                for (int x = 0; x < KS; ++x) k[x] = keys_of(tile, x);
+#pragma unroll
+                for (int t = 0; t < RT; ++t) s[t][tile] = O::scores(k, q[t]);
+            }
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
-                tree_f4 s[TILES];
-#pragma unroll
-                for (int tile = 0; tile < TILES; ++tile) {
-                    Frag k[KS];
-#pragma unroll
-                    for (int x = 0; x < KS; ++x) k[x] = keys_of(tile, x);
-                    s[tile] = O::scores(k, q[t]);
-                }
-                const unsigned long long seen = tree_seen<KEYS>(a, w, base, all_there, gone, last_page, low_of[node_of[t] - n0], words_of[node_of[t] - n0]);
-                const unsigned mine[2] = {static_cast<unsigned>(seen) >> (8 * qd), static_cast<unsigned>(seen >> 32) >> (8 * qd)};
+                seen[t] = tree_seen<KEYS>(a, w, base, all_there, gone, last_page, low_of[node_of[t] - n0], words_of[node_of[t] - n0]);
 #pragma unroll
                 for (int tile = 0; tile < TILES; ++tile)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        s[tile][i] = (mine[tile >> 1] >> (4 * (tile & 1) + i)) & 1u ? s[tile][i] * a.scale : -INFINITY;
-                tree_softmax<true>(s, m[t], l[t], o[t], 1.f);
-                unsigned bad = 0;
+                        s[t][tile][i] = (O64::shown(seen[t], tile, qd) >> O64::bit(tile, i)) & 1u ? s[t][tile][i] * a.scale : -INFINITY;
+            }
+            tree_softmax<true>(s, m, l, o, 1.f);
+            unsigned bad = 0;
 #pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    const Frag p = weights_of(s, g);
+            for (int g = 0; g < 2; ++g) {
+                Frag p[RT];
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        Frag v = values_of(dt, g);
-                        const unsigned b = O::not_finite(v);
-                        if (b) O::make_finite(v);
-                        bad |= b;
-                        o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p, o[t][dt], 0, 0, 0);
-                    }
+                for (int t = 0; t < RT; ++t) p[t] = weights_of(s[t], g);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    Frag v = values_of(dt, g);
+                    const unsigned b = O::not_finite(v);
+                    if (b) O::make_finite(v);
+                    bad |= b;
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[t], o[t][dt], 0, 0, 0);
                 }
-                if (__ballot(bad != 0))
-                    tree_odd_values<bf16, KEYS>(o[t], reinterpret_cast<const bf16*>(v_pool), page_size, a.page_shift, base, last_page, page, seen);
+            }
+            if (__ballot(bad != 0)) {
+#pragma unroll
+                for (int t = 0; t < RT; ++t)
+                    tree_odd_values<bf16, KEYS>(o[t], reinterpret_cast<const bf16*>(v_pool), page_size, a.page_shift, base, last_page, page, seen[t]);
             }
         }
         page = page_next;
