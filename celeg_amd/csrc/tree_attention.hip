@@ -214,9 +214,10 @@ struct TreeRounds {
     __device__ __forceinline__ TreeRounds(const TreeArgs& a, const TreeRequest& q, int part, int keys) {
         const int first = a.window > 0 ? max(0, q.start - a.window + 1) / keys : 0, last = q.end > 0 ? (q.end - 1) / keys : -1;
         const int total = max(last - first + 1, 0), per = (total + a.parts - 1) / a.parts;
-        r_begin = first + part * per;
-        r_end = min(last, r_begin + per - 1);
-        plain = a.window > 0 ? max(0, q.start + q.count - a.window) : 0;
+        // (the same for all lanes, as TreeRequest's)
+        r_begin = __builtin_amdgcn_readfirstlane(first + part * per);
+        r_end = __builtin_amdgcn_readfirstlane(min(last, r_begin + per - 1));
+        plain = __builtin_amdgcn_readfirstlane(a.window > 0 ? max(0, q.start + q.count - a.window) : 0);
     }
 };
 
@@ -263,6 +264,31 @@ __device__ __forceinline__ void tree_softmax(tree_f4 (&s)[RT][TILES], float (&m)
         }
         l[t] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
+}
+
+// The same for a round in which every row sees every key, without looking for the maximum: the scores become weights against the
+// running one as it stands, which is left where it is as long as no lane's weights add up to more than 2^12 (false: s is of
+// no use, the round has to be taken by tree_softmax; so the first one is).
+template <int RT, int TILES>
+__device__ __forceinline__ bool tree_weights(tree_f4 (&s)[RT][TILES], const float (&m)[RT], float (&l)[RT], float scale) {
+    float sums[RT];
+    bool in_range = true;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        tree_f4 sum = tree_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int tile = 0; tile < TILES; ++tile) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[t][tile][i] = __builtin_amdgcn_exp2f(fmaf(s[t][tile][i], scale, -m[t]));
+            sum += s[t][tile];
+        }
+        sums[t] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        in_range = in_range && sums[t] <= 4096.f;
+    }
+    if (__ballot(!in_range) != 0ull) return false;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) l[t] += sums[t];
+    return true;
 }
 
 // The keys of the round from `base` on that a row sees, a bit each (page: the lane's page of the round, `gone` if it is none).
@@ -552,9 +578,12 @@ __global__ __launch_bounds__(256, 2) void tree_rows_kernel(const TreeArgs a) {
     // A wavefront's i-th instruction fills 64 pieces of 16 bytes from piece 64 (wave + 4 i) of the keys (values) on: the lane's row of
     // keys is CH pieces long, and of values 8.  The pieces are numbered so that what hangs on the lane is the same for every i.
     constexpr bool EVEN = HD % 64 == 0;
+    const char* __restrict__ k_bytes = reinterpret_cast<const char*>(k_pool);
+    const char* __restrict__ v_bytes = reinterpret_cast<const char*>(v_pool);
+    const unsigned page_bytes = static_cast<unsigned>(2 * page_size);      // (below 2^31: checked by the host)
     const int v_dim = 8 * wave + (lane >> 3), v_key = 8 * ((lane & 7) ^ ((lane >> 3) & 7));      // dimension v_dim + 32 i
     const int k_row = 64 * wave / CH + lane / CH;                                                  // row k_row + 256 i / CH, if EVEN
-    const int k_piece = HD == 32 ? (lane & 3) ^ ((k_row >> 1) & 3) : (lane % CH) ^ (k_row & 7);
+    const int k_piece = HD == 32 ? (lane & 3) ^ ((k_row >> 1) & 3) : HD == 128 ? (lane % CH) ^ (2 * (k_row & 7)) : (lane % CH) ^ (k_row & 7);
     auto key_of_row = [](int row) { return 32 * (row >> 5) + 8 * ((row >> 2) & 3) + 4 * ((row >> 4) & 1) + (row & 3); };
     auto fetch = [&](int round, int page, Buffer& to) {       // page: valid or 0
         const int base = round * KEYS, top = top_of(round), first_page = base >> a.page_shift;
@@ -571,22 +600,23 @@ __global__ __launch_bounds__(256, 2) void tree_rows_kernel(const TreeArgs a) {
                 piece = (x % CH) ^ (row & 3);
             }
             const int key = min(base + row_key, top);
-            const __bf16* from = k_pool + __shfl(page, (key >> a.page_shift) - first_page, 64) * page_size +
-                                 (static_cast<size_t>(key & page_mask) * HD + piece * 8);
+            const char* from = k_bytes + static_cast<uint64_t>(static_cast<unsigned>(__shfl(page, (key >> a.page_shift) - first_page, 64))) * page_bytes +
+                               static_cast<unsigned>((key & page_mask) * (2 * HD) + piece * 16);
             __builtin_amdgcn_global_load_lds(TREE_GLOBAL(from), TREE_LDS(to.k + (wave + 4 * i) * 512), 16, 0, 0);
         }
         const int key = min(base + v_key, top & ~7);
-        const __bf16* from = v_pool + __shfl(page, (key >> a.page_shift) - first_page, 64) * page_size +
-                             ((static_cast<size_t>(v_dim) << a.page_shift) + (key & page_mask));
+        const char* from = v_bytes + static_cast<uint64_t>(static_cast<unsigned>(__shfl(page, (key >> a.page_shift) - first_page, 64))) * page_bytes +
+                           static_cast<unsigned>(2 * ((v_dim << a.page_shift) + (key & page_mask)));
 #pragma unroll
         for (int i = 0; i < PER; ++i)
-            __builtin_amdgcn_global_load_lds(TREE_GLOBAL(from + (static_cast<size_t>(32 * i) << a.page_shift)),
+            __builtin_amdgcn_global_load_lds(TREE_GLOBAL(from + (static_cast<unsigned>(64 * i) << a.page_shift)),
                                              TREE_LDS(to.v + (wave + 4 * i) * 512), 16, 0, 0);
     };
     // where the lane's pieces of a row lie in LDS
-    const int piece0 = EVEN ? qd ^ (c & 7) : HD == 96 ? qd ^ (c & 3) : qd ^ ((c >> 1) & 3), piece1 = (4 + qd) ^ (c & 7);
-    const int v_piece0 = qd ^ (c & 7);
-    auto k_piece_of = [&](int x) { return EVEN ? (x & 1 ? piece1 : piece0) + 8 * (x >> 1) : piece0 + 4 * x; };
+    const int v_piece0 = qd ^ (c & 7), v_piece1 = (4 + qd) ^ (c & 7);
+    auto k_piece_of = [&](int x) {
+        return HD == 128 ? (4 * x + qd) ^ (2 * (c & 7)) : HD == 64 ? (x ? v_piece1 : v_piece0) : HD == 96 ? 4 * x + (qd ^ (c & 3)) : qd ^ ((c >> 1) & 3);
+    };
     float m[RT], l[RT];
     tree_f4 o[RT][DT];
 #pragma unroll
@@ -627,7 +657,7 @@ __global__ __launch_bounds__(256, 2) void tree_rows_kernel(const TreeArgs a) {
             return *reinterpret_cast<const Frag*>(from.k + (16 * tile + c) * HD + k_piece_of(x) * 8);
         };
         auto values_of = [&](int dt, int g) {
-            return *reinterpret_cast<const Frag*>(from.v + (16 * dt + c) * KEYS + (g ? piece1 : v_piece0) * 8);
+            return *reinterpret_cast<const Frag*>(from.v + (16 * dt + c) * KEYS + (g ? v_piece1 : v_piece0) * 8);
         };
         auto weights_of = [&](const tree_f4 (&s)[TILES], int g) {
             Frag p;
@@ -639,8 +669,8 @@ __global__ __launch_bounds__(256, 2) void tree_rows_kernel(const TreeArgs a) {
             return p;
         };
         const int base = round * KEYS;
-        if (active && base >= rounds.plain && base + KEYS <= w.start && all_there) {
-            tree_f4 s[RT][TILES];
+        tree_f4 s[RT][TILES];
+        auto scores = [&]() {
 #pragma unroll
             for (int tile = 0; tile < TILES; ++tile) {
                 Frag k[KS];
@@ -649,7 +679,13 @@ __global__ __launch_bounds__(256, 2) void tree_rows_kernel(const TreeArgs a) {
 #pragma unroll
                 for (int t = 0; t < RT; ++t) s[t][tile] = O::scores(k, q[t]);
             }
-            tree_softmax<false>(s, m, l, o, a.scale);
+        };
+        if (active && base >= rounds.plain && base + KEYS <= w.start && all_there) {
+            scores();
+            if (!tree_weights(s, m, l, a.scale)) {
+                scores();
+                tree_softmax<false>(s, m, l, o, a.scale);
+            }
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 Frag p[RT];
@@ -665,16 +701,8 @@ __global__ __launch_bounds__(256, 2) void tree_rows_kernel(const TreeArgs a) {
         } else if (active) {
             // A weight of 0 times an infinity or a NaN is no 0: such values are taken out, and added for the rows that see them
             const int last_page = top_of(round) >> a.page_shift;
-            tree_f4 s[RT][TILES];
             unsigned long long seen[RT];
-#pragma unroll
-            for (int tile = 0; tile < TILES; ++tile) {
-                Frag k[KS];
-#pragma unroll
-                for (int x = 0; x < KS; ++x) k[x] = keys_of(tile, x);
-#pragma unroll
-                for (int t = 0; t < RT; ++t) s[t][tile] = O::scores(k, q[t]);
-            }
+            scores();
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
                 seen[t] = tree_seen<KEYS>(a, w, base, all_there, gone, last_page, low_of[node_of[t] - n0], words_of[node_of[t] - n0]);
