@@ -421,7 +421,7 @@ __global__ __launch_bounds__(256, 2) void tree_few_kernel(const TreeArgs a) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[t][dt] = tree_f4{0.f, 0.f, 0.f, 0.f};
     }
-    for (int round = rounds.r_begin + wave; round <= rounds.r_end; round += 4) {
+    for (int round = rounds.r_begin + (tid >> 6); round <= rounds.r_end; round += 4) {
         const int base = round * KEYS, top = min(base + KEYS, w.end) - 1;
         const int first_page = base >> a.page_shift, last_page = top >> a.page_shift;
         int page = w.pages[min(first_page + lane, last_page)];
