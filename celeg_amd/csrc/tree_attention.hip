@@ -527,28 +527,39 @@ __global__ __launch_bounds__(256, 2) void tree_few_kernel(const TreeArgs a) {
     }
 }
 
-// ---- many rows, bfloat16: the keys and values of a round are staged in LDS for the four wavefronts, each of which has 16 RT
-// rows of its own.  The next round travels straight from memory to the other of two buffers while the current one is worked on.
-// Keys lie in LDS in the order of the score tiles; the 16-byte pieces of a row change places by the row's number, so that eight
-// neighbouring lanes, which read the same piece of as many rows, read from all banks.
+// ---- many rows, bfloat16: the keys and values of a round are staged in LDS for the NW wavefronts, each of which has 16 RT rows of
+// its own.  Rounds travel straight from memory to one of NB buffers, NB - 1 ahead of the one that is worked on.
+// Keys lie in LDS in the order of the score tiles; the 16-byte pieces of a row change places by the row's number, so that the lanes
+// that are served together, which read the same piece of as many rows, read from all banks.
 #define TREE_GLOBAL(p) reinterpret_cast<const __attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(p))
 #define TREE_LDS(p) reinterpret_cast<__attribute__((address_space(3))) void*>(reinterpret_cast<uintptr_t>(p))
+#define TREE_PAGES 1024          // entries of a request's table row that are in LDS at a time
 
-template <int HD, int RT>
-__global__ __launch_bounds__(256, 2) void tree_rows_kernel(const TreeArgs a) {
+template <int N>
+__device__ __forceinline__ void tree_wait_loads() {        // at most N of the wavefront's loads are still on their way
+    static_assert(N < 64, "what the counter holds");
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+
+template <int HD, int RT, int NW, int NB>
+__global__ __launch_bounds__(64 * NW, 2) void tree_rows_kernel(const TreeArgs a) {
     // (rounds of 64 keys for any head size: staged keys cost no registers)
     using O = TreeOps<bf16, HD>;
     using O64 = TreeOps<bf16, 64>;
     using Frag = tree_bf16x8;
-    constexpr int KEYS = 64, TILES = 4, KS = O::KS, DT = O::DT, ROWS = 64 * RT, CH = HD / 8, PER = HD / 32;
+    constexpr int KEYS = 64, TILES = 4, KS = O::KS, DT = O::DT, ROWS = 16 * RT * NW, CH = HD / 8, THREADS = 64 * NW;
+    constexpr int LOADS = HD / 8, PER = (LOADS + NW - 1) / NW;      // of keys, and of values, a round: 1 KB each
     struct Buffer {
         __bf16 k[KEYS * HD];
         __bf16 v[HD * KEYS];
     };
-    __shared__ __align__(1024) Buffer buffers[2];
+    extern __shared__ __align__(1024) char tree_lds[];
+    Buffer* const buffers = reinterpret_cast<Buffer*>(tree_lds);       // [NB]
     __shared__ int up[TREE_MAX_NODES];
-    __shared__ unsigned long long words_of[ROWS][TREE_MAX_NODES / 64];
-    __shared__ int low_of[ROWS];
+    __shared__ unsigned long long words_of[ROWS < TREE_MAX_NODES ? ROWS : TREE_MAX_NODES][TREE_MAX_NODES / 64];
+    __shared__ int low_of[ROWS < TREE_MAX_NODES ? ROWS : TREE_MAX_NODES];
+    __shared__ int page_list[TREE_PAGES + 1];
+    __shared__ int any_gone;
     const int spread = (a.units + 7) & ~7, block = blockIdx.x / spread, unit = blockIdx.x % spread;
     if (unit >= a.units) return;
     const int kvh = unit % a.kv_heads, part = unit / a.kv_heads % a.parts, r = unit / (a.kv_heads * a.parts);
@@ -562,55 +573,73 @@ __global__ __launch_bounds__(256, 2) void tree_rows_kernel(const TreeArgs a) {
     const size_t head_block = per_head * (static_cast<size_t>(a.layer) * a.kv_heads + kvh);
     const __bf16* __restrict__ k_pool = static_cast<const __bf16*>(a.k_pool) + head_block;
     const __bf16* __restrict__ v_pool = static_cast<const __bf16*>(a.v_pool) + head_block;
+    const char* __restrict__ k_bytes = reinterpret_cast<const char*>(k_pool);
+    const char* __restrict__ v_bytes = reinterpret_cast<const char*>(v_pool);
+    const unsigned page_bytes = static_cast<unsigned>(2 * page_size);      // (below 2^31: checked by the host)
     const int page_mask = a.page_tokens - 1;
     Frag q[RT][KS];
     int node_of[RT];
     tree_queries<bf16, HD, RT>(a, w, kvh, j0, q, node_of);
     const int n0 = b0 / a.group, n1 = min(b0 + ROWS - 1, w.rows - 1) / a.group;
-    tree_ways<256>(a, w, n0, n1, up, words_of, low_of);
+    if (tid == 0) any_gone = 0;
+    tree_ways<THREADS>(a, w, n0, n1, up, words_of, low_of);
     const TreeRounds rounds(a, w, part, KEYS);
 
-    auto top_of = [&](int round) { return min(round * KEYS + KEYS, w.end) - 1; };
-    auto pages_of = [&](int round) {       // the lane's page of a round
-        const int first_page = round * KEYS >> a.page_shift;
-        return w.pages[min(first_page + lane, top_of(round) >> a.page_shift)];
+    // ---- the part's pages: whether all are there, and the first of them in LDS
+    const int last_page = rounds.r_end >= rounds.r_begin ? (min(rounds.r_end * KEYS + KEYS, w.end) - 1) >> a.page_shift : 0;
+    const int span = max(TREE_PAGES * a.page_tokens / KEYS, 1);        // rounds that the list serves
+    int list_round = rounds.r_begin, list_page = 0;
+    auto fill_list = [&](int round) {
+        list_round = round;
+        list_page = round * KEYS >> a.page_shift;
+        for (int i = tid; i <= TREE_PAGES; i += THREADS) {
+            const int page = w.pages[min(list_page + i, last_page)];
+            page_list[i] = page >= 0 && page < a.n_pages ? page : 0;
+        }
     };
-    // A wavefront's i-th instruction fills 64 pieces of 16 bytes from piece 64 (wave + 4 i) of the keys (values) on: the lane's row of
-    // keys is CH pieces long, and of values 8.  The pieces are numbered so that what hangs on the lane is the same for every i.
-    constexpr bool EVEN = HD % 64 == 0;
-    const char* __restrict__ k_bytes = reinterpret_cast<const char*>(k_pool);
-    const char* __restrict__ v_bytes = reinterpret_cast<const char*>(v_pool);
-    const unsigned page_bytes = static_cast<unsigned>(2 * page_size);      // (below 2^31: checked by the host)
-    const int v_dim = 8 * wave + (lane >> 3), v_key = 8 * ((lane & 7) ^ ((lane >> 3) & 7));      // dimension v_dim + 32 i
-    const int k_row = 64 * wave / CH + lane / CH;                                                  // row k_row + 256 i / CH, if EVEN
+    if (rounds.r_begin <= rounds.r_end) {
+        fill_list(rounds.r_begin);
+        bool gone = false;
+        for (int i = (rounds.r_begin * KEYS >> a.page_shift) + tid; i <= last_page; i += THREADS) gone |= w.pages[i] < 0 || w.pages[i] >= a.n_pages;
+        if (gone) any_gone = 1;
+    }
+    __syncthreads();
+    const bool all_there = __builtin_amdgcn_readfirstlane(any_gone) == 0;
+
+    // The load number wave + NW i of the keys (values) fills 64 pieces of 16 bytes from piece 64 (wave + NW i) on: the lane's row of
+    // keys is CH pieces long, and of values 8.  What hangs on the lane is the same for every i, but for heads of 96.
+    const int v_dim = 8 * wave + (lane >> 3), v_key = 8 * ((lane & 7) ^ ((lane >> 3) & 7));      // dimension v_dim + 8 NW i
+    const int k_row = (64 * wave + lane) / CH;                                                     // row k_row + 64 NW / CH i
     const int k_piece = HD == 32 ? (lane & 3) ^ ((k_row >> 1) & 3) : HD == 128 ? (lane % CH) ^ (2 * (k_row & 7)) : (lane % CH) ^ (k_row & 7);
     auto key_of_row = [](int row) { return 32 * (row >> 5) + 8 * ((row >> 2) & 3) + 4 * ((row >> 4) & 1) + (row & 3); };
-    auto fetch = [&](int round, int page, Buffer& to) {       // page: valid or 0
-        const int base = round * KEYS, top = top_of(round), first_page = base >> a.page_shift;
+    auto fetch = [&](int round, Buffer& to) {
+        const int base = round * KEYS, top = min(base + KEYS, w.end) - 1;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
+            if (LOADS % NW && wave + NW * i >= LOADS) break;
             int row_key, piece;
-            if (EVEN || PER == 1) {
-                // (rows 16 apart at 128 values: tiles of 4 keys further on, or 32; rows 32 apart at 64: 32)
-                row_key = key_of_row(k_row) + (HD == 128 ? 32 * (i >> 1) + 4 * (i & 1) : 32 * i);
+            if (HD != 96) {
+                row_key = key_of_row(k_row) + key_of_row(64 * NW / CH * i);
                 piece = k_piece;
             } else {
-                const int x = (wave + 4 * i) * 64 + lane, row = x / CH;
+                const int x = (wave + NW * i) * 64 + lane, row = x / CH;
                 row_key = key_of_row(row);
                 piece = (x % CH) ^ (row & 3);
             }
             const int key = min(base + row_key, top);
-            const char* from = k_bytes + static_cast<uint64_t>(static_cast<unsigned>(__shfl(page, (key >> a.page_shift) - first_page, 64))) * page_bytes +
+            const char* from = k_bytes + static_cast<uint64_t>(static_cast<unsigned>(page_list[(key >> a.page_shift) - list_page])) * page_bytes +
                                static_cast<unsigned>((key & page_mask) * (2 * HD) + piece * 16);
-            __builtin_amdgcn_global_load_lds(TREE_GLOBAL(from), TREE_LDS(to.k + (wave + 4 * i) * 512), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds(TREE_GLOBAL(from), TREE_LDS(to.k + (wave + NW * i) * 512), 16, 0, 0);
         }
         const int key = min(base + v_key, top & ~7);
-        const char* from = v_bytes + static_cast<uint64_t>(static_cast<unsigned>(__shfl(page, (key >> a.page_shift) - first_page, 64))) * page_bytes +
+        const char* from = v_bytes + static_cast<uint64_t>(static_cast<unsigned>(page_list[(key >> a.page_shift) - list_page])) * page_bytes +
                            static_cast<unsigned>(2 * ((v_dim << a.page_shift) + (key & page_mask)));
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
-            __builtin_amdgcn_global_load_lds(TREE_GLOBAL(from + (static_cast<unsigned>(64 * i) << a.page_shift)),
-                                             TREE_LDS(to.v + (wave + 4 * i) * 512), 16, 0, 0);
+        for (int i = 0; i < PER; ++i) {
+            if (LOADS % NW && wave + NW * i >= LOADS) break;
+            __builtin_amdgcn_global_load_lds(TREE_GLOBAL(from + (static_cast<unsigned>(16 * NW * i) << a.page_shift)),
+                                             TREE_LDS(to.v + (wave + NW * i) * 512), 16, 0, 0);
+        }
     };
     // where the lane's pieces of a row lie in LDS
     const int v_piece0 = qd ^ (c & 7), v_piece1 = (4 + qd) ^ (c & 7);
@@ -626,31 +655,24 @@ __global__ __launch_bounds__(256, 2) void tree_rows_kernel(const TreeArgs a) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[t][dt] = tree_f4{0.f, 0.f, 0.f, 0.f};
     }
-    int page = 0, page_after = 0;
-    bool gone = false, all_there = true;
-    if (rounds.r_begin <= rounds.r_end) {
-        page = pages_of(rounds.r_begin);
-        gone = page < 0 || page >= a.n_pages;
-        all_there = __ballot(gone) == 0ull;
-        page = gone ? 0 : page;
-        fetch(rounds.r_begin, page, buffers[0]);
-        if (rounds.r_begin < rounds.r_end) page_after = pages_of(rounds.r_begin + 1);
-    }
+#pragma unroll
+    for (int i = 0; i < NB - 1; ++i)
+        if (rounds.r_begin + i <= rounds.r_end) fetch(rounds.r_begin + i, buffers[i]);
     int cur = 0;
-    for (int round = rounds.r_begin; round <= rounds.r_end; ++round, cur ^= 1) {
-        // the round has arrived, for all wavefronts, and nobody reads the other buffer any more
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    for (int round = rounds.r_begin; round <= rounds.r_end; ++round, cur = cur + 1 == NB ? 0 : cur + 1) {
+        // the round has arrived, for all wavefronts, and nobody reads the buffer of the one before any more
+        if (NB > 2 && LOADS % NW == 0 && round + NB - 2 <= rounds.r_end) tree_wait_loads<(NB - 2) * 2 * PER>();
+        else tree_wait_loads<0>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        bool gone_next = false, there_next = true;
-        int page_next = 0;
-        if (round < rounds.r_end) {
-            page_next = page_after;
-            gone_next = page_next < 0 || page_next >= a.n_pages;
-            there_next = __ballot(gone_next) == 0ull;
-            page_next = gone_next ? 0 : page_next;
-            fetch(round + 1, page_next, buffers[cur ^ 1]);
-            if (round + 1 < rounds.r_end) page_after = pages_of(round + 2);
+        const int ahead = round + NB - 1;
+        if (ahead <= rounds.r_end) {
+            if (ahead >= list_round + span) {       // (everybody has read what it needs of the list: the barrier)
+                fill_list(ahead);
+                __syncthreads();
+            }
+            fetch(ahead, buffers[cur == 0 ? NB - 1 : cur - 1]);
         }
         const Buffer& from = buffers[cur];
         auto keys_of = [&](int tile, int x) {
@@ -700,12 +722,16 @@ __global__ __launch_bounds__(256, 2) void tree_rows_kernel(const TreeArgs a) {
             }
         } else if (active) {
             // A weight of 0 times an infinity or a NaN is no 0: such values are taken out, and added for the rows that see them
-            const int last_page = top_of(round) >> a.page_shift;
+            const int first_page = base >> a.page_shift, end_page = (min(base + KEYS, w.end) - 1) >> a.page_shift;
+            int page = w.pages[min(first_page + lane, end_page)];
+            const bool gone = page < 0 || page >= a.n_pages;
+            page = gone ? 0 : page;
+            const bool round_there = __ballot(gone) == 0ull;
             unsigned long long seen[RT];
             scores();
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
-                seen[t] = tree_seen<KEYS>(a, w, base, all_there, gone, last_page, low_of[node_of[t] - n0], words_of[node_of[t] - n0]);
+                seen[t] = tree_seen<KEYS>(a, w, base, round_there, gone, end_page, low_of[node_of[t] - n0], words_of[node_of[t] - n0]);
 #pragma unroll
                 for (int tile = 0; tile < TILES; ++tile)
 #pragma unroll
@@ -732,12 +758,9 @@ __global__ __launch_bounds__(256, 2) void tree_rows_kernel(const TreeArgs a) {
             if (__ballot(bad != 0)) {
 #pragma unroll
                 for (int t = 0; t < RT; ++t)
-                    tree_odd_values<bf16, KEYS>(o[t], reinterpret_cast<const bf16*>(v_pool), page_size, a.page_shift, base, last_page, page, seen[t]);
+                    tree_odd_values<bf16, KEYS>(o[t], reinterpret_cast<const bf16*>(v_pool), page_size, a.page_shift, base, end_page, page, seen[t]);
             }
         }
-        page = page_next;
-        gone = gone_next;
-        all_there = there_next;
     }
     if (!active) return;
 #pragma unroll
@@ -746,6 +769,14 @@ __global__ __launch_bounds__(256, 2) void tree_rows_kernel(const TreeArgs a) {
         const int j = j0 + 16 * t + c;
         if (j < w.rows) tree_store<bf16, HD>(a, w.first + node_of[t], kvh * a.group + j % a.group, part, qd, m[t], l[t], o[t]);
     }
+}
+
+template <int HD, int RT, int NW, int NB>
+static void launch_tree_rows(const TreeArgs& a, dim3 grid, hipStream_t stream) {
+    constexpr int bytes = NB * 2 * 64 * HD * 2;
+    // (more than 64 KB a workgroup has to be asked for; the same call every time, which costs nothing next to the launch)
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(tree_rows_kernel<HD, RT, NW, NB>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    tree_rows_kernel<HD, RT, NW, NB><<<grid, dim3(64 * NW), bytes, stream>>>(a);
 }
 
 // The parts of a node and query head: out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.  A wavefront each; four to a workgroup.
@@ -778,15 +809,24 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeArgs a) {
         if (lane + 64 * e < HD) to[lane + 64 * e] = from_float<T>(o[e] / sum);
 }
 
-// The form of a launch: rows of a workgroup, and keys of a round.
+// The form of a launch: whether keys are staged, row tiles of a wavefront, rows of a workgroup, keys of a round, and workgroups
+// that a compute unit holds.
+//   Up to 32 rows nothing is gained by staging: four wavefronts read 16 or 32 rows' keys themselves.  Above, staged: 64 rows by four
+// wavefronts, 128 by four with two row tiles each, and more by eight, which read every key once for 256 rows, from four buffers (16
+// trees of 64 nodes behind 12,001 to 16,384 tokens, 32 heads of 128 on 8: 378 us, in workgroups of 128 rows 437; heads of 64 252 and
+// 278; 8 trees of 64 behind 8,192 tokens, heads of 64: 72 and 75).
 struct TreeForm {
     bool staged;
-    int tiles, rows, keys;
+    int tiles, rows, keys, resident;
 };
 static TreeForm tree_form(int dtype, int head_dim, int rows) {
-    if (dtype == CELEG_BF16 && rows > 32) return rows <= 64 ? TreeForm{true, 1, 64, 64} : TreeForm{true, 2, 128, 64};
+    if (dtype == CELEG_BF16 && rows > 32) {
+        if (rows <= 64) return {true, 1, 64, 64, 2};
+        if (rows <= 128) return {true, 2, 128, 64, 2};
+        return {true, 2, 256, 64, 1};
+    }
     const int tiles = rows <= 16 || (dtype != CELEG_BF16 && head_dim > 64) ? 1 : 2;
-    return {false, tiles, 16 * tiles, dtype == CELEG_BF16 && head_dim <= 64 ? 64 : 32};
+    return {false, tiles, 16 * tiles, dtype == CELEG_BF16 && head_dim <= 64 ? 64 : 32, 2};
 }
 
 // Whether the matrix cores take these sizes.
@@ -794,13 +834,15 @@ extern "C" int celeg_tree_attention_fast_ok(int head_dim, int page_tokens) {
     return (head_dim == 32 || head_dim == 64 || head_dim == 96 || head_dim == 128) && page_tokens >= 16 && (page_tokens & (page_tokens - 1)) == 0;
 }
 
-// Parts that the contexts are cut into: about two workgroups a compute unit, each wavefront with a round at least.
+// Parts that the contexts are cut into: as many workgroups as the chip holds at a time, each wavefront (each workgroup that stages:
+// two) with a round at least.  More of them cost more to join than an even end gains (as above, 512 workgroups of 128 rows: 446 us, 640:
+// 470, 1,024: 485).
 extern "C" int celeg_tree_attention_parts(int dtype, int head_dim, int requests, int kv_heads, int group, int max_nodes, int max_context) {
     const int rows = max_nodes * group;
     const TreeForm form = tree_form(dtype, head_dim, rows);
     const long long groups = static_cast<long long>(requests) * kv_heads * ((rows + form.rows - 1) / form.rows);
     const long long rounds = (static_cast<long long>(max_context) + max_nodes + form.keys - 1) / form.keys;
-    return static_cast<int>(std::max(1LL, std::min({(512 + groups - 1) / groups, form.staged ? (rounds + 1) / 2 : (rounds + 3) / 4, 64LL})));
+    return static_cast<int>(std::max(1LL, std::min({(256 * form.resident + groups - 1) / groups, form.staged ? (rounds + 1) / 2 : (rounds + 3) / 4, 64LL})));
 }
 
 extern "C" int celeg_tree_attention_fast(const void* q, int ldq, int dtype, const void* k_pool, const void* v_pool, int n_pages, int n_layers,
@@ -850,8 +892,9 @@ extern "C" int celeg_tree_attention_fast(const void* q, int ldq, int dtype, cons
         constexpr bool B = std::is_same<T, bf16>::value;
         if (form.staged) {
             if constexpr (B) {
-                if (form.tiles == 2) tree_rows_kernel<HD, 2><<<grid, dim3(256), 0, stream>>>(a);
-                else tree_rows_kernel<HD, 1><<<grid, dim3(256), 0, stream>>>(a);
+                if (form.rows == 256) launch_tree_rows<HD, 2, 8, 4>(a, grid, stream);
+                else if (form.tiles == 2) launch_tree_rows<HD, 2, 4, 2>(a, grid, stream);
+                else launch_tree_rows<HD, 1, 4, 2>(a, grid, stream);
             }
         } else if (form.tiles == 2) {
             if constexpr (B || HD <= 64) tree_few_kernel<T, HD, 2><<<grid, dim3(256), 0, stream>>>(a);
