@@ -116,6 +116,18 @@ class CacheManager(_Host):
     def covers(self, slot: int, start_pos: int, n_new: int) -> bool:
         return self._call("covers", slot, start_pos, n_new)
 
+    def fork(self, slot: int, length: int) -> Optional[int]:
+        """A request that goes on from the first ``length`` tokens of ``slot``: their pages are shared until one of the
+        two prepares to write to one.  None: every slot is taken."""
+        other = self._call("fork", slot, length)
+        return None if other < 0 else other
+
+    def truncate(self, slot: int, length: int) -> None:
+        self._call("truncate", slot, length)
+
+    def holds(self, slot: int, start_pos: int, n: int) -> bool:
+        return self._call("holds", slot, start_pos, n)
+
     def pages_needed(self, slot: int, start_pos: int, n_new: int) -> List[int]:
         return self._call("pages_needed", slot, start_pos, n_new)
 

@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import argparse
 import json
+import math
 import os
 import sys
 import tempfile
@@ -44,6 +45,9 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--dump-logits", default=None, metavar="FILE.f32",
                     help="write the logits after the prompt as raw 32-bit floats")
     ap.add_argument("--print-top", type=int, default=0, metavar="N")
+    ap.add_argument("--prompt-logprobs", type=int, default=None, metavar="N",
+                    help="judge the prompt itself: for every token behind the first its log probability and rank and the N (up to 128) "
+                         "most likely tokens in its place, and the perplexity, on stderr")
     ap.add_argument("--tokens-only", action="store_true", help="print the prompt's ids and exit")
     ap.add_argument("--runtime-tokens", action="store_true",
                     help="print CELEG_GENERATED_TOKEN_IDS=[...]")
@@ -116,6 +120,8 @@ def validate(args, ap) -> None:
             or args.benchmark_warmup < 0 or args.benchmark_prefill_tokens < 0 \
             or args.prefill_chunk <= 0 or args.batch <= 0 or args.page_tokens <= 0:
         ap.error("invalid numeric argument")
+    if args.prompt_logprobs is not None and not 0 <= args.prompt_logprobs <= 128:
+        ap.error("--prompt-logprobs must be in [0, 128]")
     if args.attention_chunk_tokens not in (0, 64, 256, 1024):
         ap.error("--attention-chunk-tokens must be 64, 256 or 1024")
 
@@ -222,6 +228,9 @@ def run(args) -> int:
         _reports(args, engine)
         return 0
 
+    if args.prompt_logprobs is not None:
+        _judge(lm, prompt, min(args.prompt_logprobs, lm.native.logit_width), min(args.prefill_chunk, budget))
+
     generation = GenerationConfig(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
                                   repetition_penalty=args.repetition_penalty, seed=args.seed)
     rid = engine.submit(prompt, RequestOptions(max_new_tokens=max(args.max_new_tokens, 1),
@@ -257,6 +266,18 @@ def run(args) -> int:
     if tmp is not None:
         tmp.cleanup()
     return 0
+
+
+def _judge(lm, prompt, top, portion) -> None:
+    """--prompt-logprobs: a line for every token behind the first, then the perplexity."""
+    judged = lm.score(prompt, top=top, portion=portion)
+    for i, target in enumerate(prompt[1:]):
+        best = " ".join(f"{t}:{p:.4f}" for t, p in zip(judged.top_ids[i].tolist(), judged.top_logprobs[i].tolist()))
+        print(f"logprob[{i + 1}] token={target} logprob={judged.logprobs[i, 0]:.4f} rank={int(judged.ranks[i, 0])} "
+              f"entropy={judged.entropy[i]:.4f}" + (f" top={best}" if best else ""), file=sys.stderr)
+    if len(prompt) > 1:
+        mean = judged.logprobs.double().mean().item()
+        print(f"prompt.mean_logprob={mean:.6f}\nprompt.perplexity={math.exp(-mean):.6f}", file=sys.stderr)
 
 
 def _reports(args, engine, request_id=None) -> None:

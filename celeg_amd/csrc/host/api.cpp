@@ -8,6 +8,7 @@
 #include <set>
 #include <algorithm>
 
+#include "branch.hpp"
 #include "engine.hpp"
 #include "model.hpp"
 
@@ -28,6 +29,7 @@ struct ModelSession {
 struct celeg_model {
     std::unique_ptr<LoadedModel> owned;
     LoadedModel* lm = nullptr;
+    DeviceBuffer logprob_block;     // what a step's logits say about tokens, on its way to the host
     PinnedBuffer logits_stage;      // few rows of logits come to the host through pinned memory
     std::unique_ptr<ModelSession> session;
     // (the session's sampler points into the model's runtime: it goes first)
@@ -54,6 +56,10 @@ celeg_status guarded(F&& body, std::string* also = nullptr) {
         body();
         return CELEG_OK;
     } catch (const ConfigError& e) {
+        g_error = e.what();
+        if (also) *also = g_error;
+        return CELEG_INVALID_ARGUMENT;
+    } catch (const ArgumentError& e) {
         g_error = e.what();
         if (also) *also = g_error;
         return CELEG_INVALID_ARGUMENT;
@@ -371,6 +377,7 @@ const char* celeg_model_describe(celeg_model* model) {
                 .set("logit_width", lm.model->logit_width()).set("max_context", lm.cache->max_context)
                 .set("page_tokens", lm.cache->page_tokens).set("max_requests", lm.cache->max_requests)
                 .set("max_batched_tokens", lm.runner->max_batched_tokens).set("graph_safe", lm.model->graph_safe())
+                .set("takes_trees", lm.model->takes_trees())
                 .set("dtype", dtype_name(lm.rt->dtype)).set("weights", lm.model->weight_count())
                 .set("kv_bytes_per_token", lm.cache->layout.kv_bytes_per_token(dtype_size(lm.rt->dtype)))
                 .set("eos_token_ids", Json::array_of(lm.model->spec.eos_token_ids))
@@ -420,27 +427,118 @@ const char* celeg_model_cache_state(celeg_model* model) {
                     .set("memory", c.memory_bytes()).dump());
 }
 
+celeg_status celeg_model_fork_slot(celeg_model* model, int32_t slot, int32_t length, int32_t* new_slot) {
+    if (!model || !new_slot) {
+        g_error = "celeg_model_fork_slot: null argument";
+        return CELEG_INVALID_ARGUMENT;
+    }
+    return guarded([&] { *new_slot = model->lm->cache->fork(slot, length); });
+}
+
+celeg_status celeg_model_keep(celeg_model* model, int32_t slot, int32_t start, const int32_t* places, int32_t n) {
+    if (!model || n < 0 || (n > 0 && !places)) {
+        g_error = "celeg_model_keep: null argument or negative count";
+        return CELEG_INVALID_ARGUMENT;
+    }
+    return guarded([&] { model->lm->runner->keep(slot, start, n ? std::vector<int>(places, places + n) : std::vector<int>()); });
+}
+
+// The entries of a step as the C interface gives them, and how many logits they want.
+static std::vector<StepEntry> step_entries(int32_t n_entries, const int32_t* slot, const int32_t* start_pos, const int32_t* n_tokens,
+                                           const int32_t* tokens, const int32_t* parents, const int32_t* n_want, const int32_t* want,
+                                           size_t* wanted) {
+    std::vector<StepEntry> entries(static_cast<size_t>(n_entries));
+    size_t t = 0, w = 0;
+    for (int i = 0; i < n_entries; ++i) {
+        StepEntry& e = entries[static_cast<size_t>(i)];
+        e.slot = slot[i];
+        e.start_pos = start_pos[i];
+        if (n_tokens[i] < 0 || n_want[i] < 0 || (n_want[i] > 0 && !want)) throw StepError("step: negative count");
+        e.tokens.assign(tokens + t, tokens + t + n_tokens[i]);
+        if (parents) e.parents.assign(parents + t, parents + t + n_tokens[i]);
+        e.want.assign(want + w, want + w + n_want[i]);
+        t += static_cast<size_t>(n_tokens[i]);
+        w += static_cast<size_t>(n_want[i]);
+    }
+    *wanted = w;
+    return entries;
+}
+
 celeg_status celeg_model_step(celeg_model* model, int32_t n_entries, const int32_t* slot, const int32_t* start_pos,
                               const int32_t* n_tokens, const int32_t* tokens, const int32_t* n_want, const int32_t* want,
                               float* logits, size_t capacity) {
+    return celeg_model_step_tree(model, n_entries, slot, start_pos, n_tokens, tokens, nullptr, n_want, want, logits, capacity);
+}
+
+celeg_status celeg_model_step_logprobs(celeg_model* model, int32_t n_entries, const int32_t* slot, const int32_t* start_pos,
+                                       const int32_t* n_tokens, const int32_t* tokens, const int32_t* parents, const int32_t* n_want,
+                                       const int32_t* want, const int32_t* targets, int32_t per_row, int32_t top, float* logprobs,
+                                       int32_t* ranks, float* entropy, int32_t* top_ids, float* top_logprobs) {
+    if (!model || n_entries < 0 || (n_entries > 0 && (!slot || !start_pos || !n_tokens || !tokens || !n_want)) || per_row < 0 || top < 0 ||
+        (per_row > 0 && (!targets || !logprobs || !ranks)) || !entropy || (top > 0 && (!top_ids || !top_logprobs))) {
+        g_error = "celeg_model_step_logprobs: null argument or negative count";
+        return CELEG_INVALID_ARGUMENT;
+    }
+    return guarded([&] {
+        size_t wanted = 0;
+        const std::vector<StepEntry> entries = step_entries(n_entries, slot, start_pos, n_tokens, tokens, parents, n_want, want, &wanted);
+        LoadedModel& lm = *model->lm;
+        TokenLogprobs a;
+        a.rows = static_cast<long long>(wanted);
+        a.vocab = a.row_stride = lm.model->logit_width();
+        a.per_row = per_row;
+        a.top = top;
+        // (what the arguments ask for is checked before the step runs: a step that has run has advanced its requests)
+        const size_t workspace = token_logprobs_workspace(a);
+        const Tensor logits = lm.runner->step(entries);
+        if (!wanted) {
+            CELEG_HIP(hipStreamSynchronize(lm.stream));
+            return;
+        }
+        a.logits = logits.data;
+        a.dtype = logits.dtype;
+        a.row_stride = logits.row_stride();
+        // One block of device memory for what comes back (32-bit each), the targets and the workspace: 16 bytes apart
+        const size_t n = wanted, given = n * static_cast<size_t>(per_row), best = n * static_cast<size_t>(top);
+        const size_t back = 2 * given + n + 2 * best, at_workspace = (back + given + 3) / 4 * 16;
+        DeviceBuffer& block = model->logprob_block;
+        if (block.bytes() < at_workspace + workspace) block = DeviceBuffer(std::max(2 * block.bytes(), at_workspace + workspace));
+        float* out = block.as<float>();
+        int* device_targets = reinterpret_cast<int*>(out + back);
+        if (given) CELEG_HIP(hipMemcpyAsync(device_targets, targets, given * 4, hipMemcpyHostToDevice, lm.stream));
+        a.tokens = given ? device_targets : nullptr;
+        a.logprobs = out;
+        a.ranks = reinterpret_cast<int*>(out + given);
+        a.entropy = out + 2 * given;
+        a.top_ids = reinterpret_cast<int*>(out + 2 * given + n);
+        a.top_logprobs = out + 2 * given + n + best;
+        token_logprobs(a, block.as<char>() + at_workspace, workspace, lm.stream);
+        std::vector<float> host(back);
+        CELEG_HIP(hipMemcpyAsync(host.data(), out, back * 4, hipMemcpyDeviceToHost, lm.stream));
+        CELEG_HIP(hipStreamSynchronize(lm.stream));
+        const float* from = host.data();
+        auto give = [&](void* to, size_t count) {
+            if (count) std::memcpy(to, from, count * 4);
+            from += count;
+        };
+        give(logprobs, given);
+        give(ranks, given);
+        give(entropy, n);
+        give(top_ids, best);
+        give(top_logprobs, best);
+    });
+}
+
+celeg_status celeg_model_step_tree(celeg_model* model, int32_t n_entries, const int32_t* slot, const int32_t* start_pos,
+                                   const int32_t* n_tokens, const int32_t* tokens, const int32_t* parents, const int32_t* n_want,
+                                   const int32_t* want, float* logits, size_t capacity) {
     if (!model || n_entries < 0 || (n_entries > 0 && (!slot || !start_pos || !n_tokens || !tokens || !n_want))) {
         g_error = "celeg_model_step: null argument";
         return CELEG_INVALID_ARGUMENT;
     }
     return guarded([&] {
-        std::vector<StepEntry> entries(static_cast<size_t>(n_entries));
-        size_t t = 0, w = 0, wanted = 0;
-        for (int i = 0; i < n_entries; ++i) {
-            StepEntry& e = entries[static_cast<size_t>(i)];
-            e.slot = slot[i];
-            e.start_pos = start_pos[i];
-            if (n_tokens[i] < 0 || n_want[i] < 0 || (n_want[i] > 0 && !want)) throw StepError("step: negative count");
-            e.tokens.assign(tokens + t, tokens + t + n_tokens[i]);
-            e.want.assign(want + w, want + w + n_want[i]);
-            t += static_cast<size_t>(n_tokens[i]);
-            w += static_cast<size_t>(n_want[i]);
-            wanted += static_cast<size_t>(n_want[i]);
-        }
+        size_t wanted = 0;
+        const std::vector<StepEntry> entries = step_entries(n_entries, slot, start_pos, n_tokens, tokens, parents, n_want, want, &wanted);
         LoadedModel& lm = *model->lm;
         // (checked before the step runs: a step that has run has advanced its requests)
         if (wanted && !logits) throw StepError("step: logits are wanted and there is no buffer for them");

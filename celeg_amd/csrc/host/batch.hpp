@@ -25,6 +25,9 @@ struct StepEntry {
     int start_pos = 0;            // position of tokens[0] in the request's sequence
     std::vector<int> tokens;      // {TOKEN_FROM_DEVICE}: the token the request sampled last, taken on the device
     std::vector<int> want;        // indices into tokens whose logits are wanted
+    // drafted tokens that branch: of each token the index of its parent, lower than its own, -1: it follows the start itself.
+    // Empty: every token follows the one before it.
+    std::vector<int> parents;
 };
 
 // (slot, logical page, physical page)
@@ -48,6 +51,10 @@ struct StepBatch {
     std::vector<int> entry_order;          // which entry each sequence of the layout is
     int *token_ids = nullptr, *positions = nullptr, *token_seq = nullptr, *token_slot = nullptr;
     int *cu_seqlens = nullptr, *seq_slot = nullptr, *seq_start = nullptr, *logit_rows = nullptr;
+    // a step with trees of drafted tokens: where a row's key and value lie (`positions` are its start plus its depth then, by which
+    // it is rotated), its parent in its tree, and the most rows of a tree
+    int *tree_places = nullptr, *tree_parents = nullptr;
+    int max_tree_nodes = 0;
     std::vector<int*> table_updates;
     std::vector<int> table_update_caps;
     // host copies, for parts that plan on the host

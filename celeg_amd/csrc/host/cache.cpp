@@ -3,6 +3,8 @@
 #include <algorithm>
 #include <set>
 
+#include "branch.hpp"
+
 namespace celeg {
 
 // ---------------------------------------------------------------------------- pages
@@ -210,7 +212,17 @@ std::vector<int> CacheManager::pages_needed(int slot, int start_pos, int n_new) 
     const int top = (start_pos + n_new - 1) / page_tokens;
     std::vector<int> out;
     for (const Group& g : groups_)
-        out.push_back(std::max(0, top + 1 - static_cast<int>(g.pages[static_cast<size_t>(slot)].size())));
+        out.push_back(std::max(0, top + 1 - static_cast<int>(g.pages[static_cast<size_t>(slot)].size())) +
+                      static_cast<int>(shared_pages(g, slot, start_pos, n_new).size()));
+    return out;
+}
+
+std::vector<int> CacheManager::shared_pages(const Group& g, int slot, int start_pos, int n) const {
+    std::vector<int> out;
+    const auto& pages = g.pages[static_cast<size_t>(slot)];
+    const int end = std::min((start_pos + n - 1) / page_tokens + 1, static_cast<int>(pages.size()));
+    for (int idx = std::max(start_pos, 0) / page_tokens; idx < end; ++idx)
+        if (pages[static_cast<size_t>(idx)] >= 0 && g.pool.holders(pages[static_cast<size_t>(idx)]) > 1) out.push_back(idx);
     return out;
 }
 
@@ -240,12 +252,13 @@ bool CacheManager::prepare(int slot, int start_pos, int n_new) {
     const std::vector<int> need = pages_needed(slot, start_pos, n_new);
     for (size_t g = 0; g < groups_.size(); ++g)
         if (need[g] > groups_[g].pool.n_free()) return false;
+    unshare(slot, start_pos, n_new);
     for (size_t gi = 0; gi < groups_.size(); ++gi) {
         Group& g = groups_[gi];
         std::vector<int> fresh;
-        g.pool.allocate(need[gi], fresh);
+        auto& pages = g.pages[static_cast<size_t>(slot)];
+        g.pool.allocate(std::max(0, (start_pos + n_new - 1) / page_tokens + 1 - static_cast<int>(pages.size())), fresh);
         for (int p : fresh) {
-            auto& pages = g.pages[static_cast<size_t>(slot)];
             const int idx = static_cast<int>(pages.size());
             pages.push_back(p);
             g.table_host[static_cast<size_t>(slot) * max_pages_per_request + idx] = p;
@@ -261,7 +274,7 @@ bool CacheManager::covers(int slot, int start_pos, int n_new) const {
     const int top = (start_pos + n_new - 1) / page_tokens;
     for (const Group& g : groups_) {
         const auto& pages = g.pages[static_cast<size_t>(slot)];
-        if (top >= static_cast<int>(pages.size())) return false;
+        if (top >= static_cast<int>(pages.size()) || !shared_pages(g, slot, start_pos, n_new).empty()) return false;
         const int low = g.need.window ? std::max(0, start_pos - *g.need.window + 1) : 0;
         for (int idx = low / page_tokens; idx <= top; ++idx)
             if (pages[static_cast<size_t>(idx)] < 0) return false;
@@ -270,6 +283,98 @@ bool CacheManager::covers(int slot, int start_pos, int n_new) const {
             if (pages[static_cast<size_t>(idx)] < 0) return false;
     }
     return true;
+}
+
+bool CacheManager::holds(int slot, int start_pos, int n) const {
+    if (!open_.count(slot) || start_pos < 0 || n < 0) return false;
+    for (const Group& g : groups_) {
+        const auto& pages = g.pages[static_cast<size_t>(slot)];
+        for (long long idx = start_pos / page_tokens; n > 0 && idx <= (static_cast<long long>(start_pos) + n - 1) / page_tokens; ++idx)
+            if (idx >= static_cast<long long>(pages.size()) || pages[static_cast<size_t>(idx)] < 0) return false;
+    }
+    return true;
+}
+
+bool CacheManager::unshare(int slot, int start_pos, int n) {
+    if (!open_.count(slot)) throw PageError("slot " + std::to_string(slot) + " is not open");
+    if (n <= 0) return true;
+    std::vector<std::vector<int>> shared;
+    for (const Group& g : groups_) {
+        shared.push_back(shared_pages(g, slot, start_pos, n));
+        if (static_cast<int>(shared.back().size()) > g.pool.n_free()) return false;
+    }
+    for (size_t gi = 0; gi < groups_.size(); ++gi) {
+        Group& g = groups_[gi];
+        const int count = static_cast<int>(shared[gi].size());
+        if (!count) continue;
+        std::vector<int> fresh, lists;
+        g.pool.allocate(count, fresh);
+        auto& pages = g.pages[static_cast<size_t>(slot)];
+        for (int idx : shared[gi]) lists.push_back(pages[static_cast<size_t>(idx)]);
+        lists.insert(lists.end(), fresh.begin(), fresh.end());
+        if (on_device_) {
+            const size_t bytes = lists.size() * sizeof(int);
+            if (copy_list_.bytes() < bytes) copy_list_ = DeviceBuffer(std::max<size_t>(bytes, 1024));
+            CELEG_HIP(hipMemcpyAsync(copy_list_.ptr(), lists.data(), bytes, hipMemcpyHostToDevice, stream_));
+            copy_pages(group_view(static_cast<int>(gi)), copy_list_.as<int>(), copy_list_.as<int>() + count, count, stream_);
+            CELEG_HIP(hipStreamSynchronize(stream_));      // (the lists go away)
+        }
+        for (int i = 0; i < count; ++i) {
+            const int idx = shared[gi][static_cast<size_t>(i)];
+            g.pool.release({pages[static_cast<size_t>(idx)]});
+            pages[static_cast<size_t>(idx)] = fresh[static_cast<size_t>(i)];
+            g.table_host[static_cast<size_t>(slot) * max_pages_per_request + idx] = fresh[static_cast<size_t>(i)];
+            g.add_update(slot, idx, fresh[static_cast<size_t>(i)]);
+        }
+    }
+    return true;
+}
+
+int CacheManager::fork(int slot, int length) {
+    if (!open_.count(slot)) throw PageError("slot " + std::to_string(slot) + " is not open");
+    if (length < 0 || length > open_.at(slot))
+        throw PageError("fork: slot " + std::to_string(slot) + " has pages for " + std::to_string(open_.at(slot)) + " tokens, not " +
+                        std::to_string(length));
+    const int other = open();
+    if (other < 0) return -1;
+    const int count = (length + page_tokens - 1) / page_tokens;
+    for (Group& g : groups_) {
+        const auto& from = g.pages[static_cast<size_t>(slot)];
+        auto& pages = g.pages[static_cast<size_t>(other)];
+        pages.assign(from.begin(), from.begin() + count);
+        for (int idx = 0; idx < count; ++idx) {
+            const int p = pages[static_cast<size_t>(idx)];
+            if (p < 0) continue;
+            g.pool.retain({p});
+            g.table_host[static_cast<size_t>(other) * max_pages_per_request + idx] = p;
+            g.add_update(other, idx, p);
+        }
+        g.first_live[static_cast<size_t>(other)] = std::min(g.first_live[static_cast<size_t>(slot)], count);
+    }
+    if (slot_bytes && on_device_) {
+        char* states = static_cast<char*>(state_buffer_.ptr());
+        CELEG_HIP(hipMemcpyAsync(states + static_cast<size_t>(other) * slot_bytes, states + static_cast<size_t>(slot) * slot_bytes, slot_bytes,
+                                 hipMemcpyDeviceToDevice, stream_));
+    }
+    open_[other] = length;
+    return other;
+}
+
+void CacheManager::truncate(int slot, int length) {
+    if (!open_.count(slot)) throw PageError("slot " + std::to_string(slot) + " is not open");
+    if (length < 0 || length > open_.at(slot))
+        throw PageError("truncate: slot " + std::to_string(slot) + " has pages for " + std::to_string(open_.at(slot)) + " tokens, not " +
+                        std::to_string(length));
+    const size_t count = static_cast<size_t>((length + page_tokens - 1) / page_tokens);
+    for (Group& g : groups_) {
+        auto& pages = g.pages[static_cast<size_t>(slot)];
+        for (; pages.size() > count; pages.pop_back()) {
+            if (pages.back() >= 0) g.pool.release({pages.back()});
+            g.table_host[static_cast<size_t>(slot) * max_pages_per_request + pages.size() - 1] = -1;
+        }
+        g.first_live[static_cast<size_t>(slot)] = std::min(g.first_live[static_cast<size_t>(slot)], static_cast<int>(count));
+    }
+    open_[slot] = length;
 }
 
 std::vector<std::vector<int>> CacheManager::pages_held(int slot) const {
@@ -310,27 +415,31 @@ void CacheManager::requeue_table_updates(const std::vector<std::vector<TableUpda
     }
 }
 
+KVView CacheManager::group_view(int group) const {
+    const Group& g = groups_.at(static_cast<size_t>(group));
+    KVView kv;
+    kv.k = g.k.ptr();
+    kv.v = g.v.ptr();
+    kv.dtype = dtype;
+    kv.n_layers = g.n_layers;
+    kv.table = g.table.as<int>();
+    kv.table_stride = max_pages_per_request;
+    kv.table_rows = max_requests + 1;
+    kv.page_tokens = page_tokens;
+    kv.kv_heads = g.need.kv_heads;
+    kv.head_dim = g.need.head_dim;
+    kv.v_head_dim = g.need.value_dim();
+    kv.group = group;
+    kv.n_pages = g.pool.n_pages() + 1;
+    return kv;
+}
+
 LayerCache CacheManager::layer_cache(int step) const {
     LayerCache out;
     auto it = layout.kv_of_step.find(step);
     if (it != layout.kv_of_step.end()) {
-        const Group& g = groups_.at(static_cast<size_t>(it->second.group));
-        KVView kv;
-        kv.k = g.k.ptr();
-        kv.v = g.v.ptr();
-        kv.dtype = dtype;
-        kv.layer = it->second.layer;
-        kv.n_layers = g.n_layers;
-        kv.table = g.table.as<int>();
-        kv.table_stride = max_pages_per_request;
-        kv.table_rows = max_requests + 1;
-        kv.page_tokens = page_tokens;
-        kv.kv_heads = g.need.kv_heads;
-        kv.head_dim = g.need.head_dim;
-        kv.v_head_dim = g.need.value_dim();
-        kv.group = it->second.group;
-        kv.n_pages = g.pool.n_pages() + 1;
-        out.kv = kv;
+        out.kv = group_view(it->second.group);
+        out.kv->layer = it->second.layer;
         out.writes_kv = it->second.writes;
     }
     for (const auto& r : regions_) {
@@ -361,19 +470,19 @@ int CacheManager::table_host(int group, int slot, int logical) const {
 void CacheManager::check() const {
     for (const Group& g : groups_) {
         g.pool.check();
-        std::map<int, int> seen;
+        std::map<int, int> seen, held;
         for (int slot = 0; slot < max_requests; ++slot)
             for (int p : g.pages[static_cast<size_t>(slot)]) {
                 if (p < 0) continue;
                 if (!open_.count(slot))
                     throw PageError("closed slot " + std::to_string(slot) + " still holds page " + std::to_string(p));
-                if (seen.count(p))
+                if (++held[p] > g.pool.holders(p))
                     throw PageError("page " + std::to_string(p) + " is held by slots " + std::to_string(seen[p]) + " and " +
                                     std::to_string(slot));
                 seen[p] = slot;
             }
         for (int p = 0; p < g.pool.n_pages(); ++p)
-            if ((g.pool.holders(p) > 0) != (seen.count(p) > 0))
+            if (g.pool.holders(p) != (held.count(p) ? held.at(p) : 0))
                 throw PageError("page " + std::to_string(p) + ": pool and block tables disagree");
     }
     std::set<int> free(free_slots_.begin(), free_slots_.end());

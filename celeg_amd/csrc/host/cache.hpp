@@ -135,7 +135,19 @@ public:
     // back the pages that no later token can see (window groups).  False, with no page taken,
     // if some pool has too few free pages.
     bool prepare(int slot, int start_pos, int n_new);
+    // whether the request's pages cover these positions, and none of those is shared with another request
     bool covers(int slot, int start_pos, int n_new) const;
+    // A request that goes on from the first `length` tokens of an open one, with its state as it stands.  The pages that
+    // hold them are shared until either request is about to write to one: prepare() then gives that one a copy of its own.
+    // -1: every slot is taken.
+    int fork(int slot, int length);
+    // forgets the tokens from `length` on: pages that hold none of the others are given back
+    void truncate(int slot, int length);
+    int tokens(int slot) const { return open_.count(slot) ? open_.at(slot) : 0; }      // that the request has been given pages for
+    // whether every group has a page for these positions, now
+    bool holds(int slot, int start_pos, int n) const;
+    // pages of its own for positions [start_pos, start_pos + n) as far as the request has pages for them; false: too few are free
+    bool unshare(int slot, int start_pos, int n);
     std::vector<std::vector<int>> pages_held(int slot) const;
     std::vector<int> free_pages() const;
     // Pages added to the block tables since the last call, per group, in order, at most one per
@@ -147,6 +159,7 @@ public:
     // update of the same table entry wins
     void requeue_table_updates(const std::vector<std::vector<TableUpdate>>& updates);
     LayerCache layer_cache(int step) const;
+    KVView group_view(int group) const;       // (layer 0)
     void check() const;          // no page lost, none held twice; slots free or open, never both
     Json memory_bytes() const;
     // where, inside a slot's row of bytes, the state `name` of run-order entry `step` lies
@@ -173,6 +186,8 @@ private:
     };
     struct Region { size_t offset; StateNeed need; };
     void release_passed(Group& g, int slot, int next_pos);
+    std::vector<int> shared_pages(const Group& g, int slot, int start_pos, int n) const;       // logical numbers
+    DeviceBuffer copy_list_;      // pages that a copy goes from and to
     std::vector<Group> groups_;
     std::map<std::pair<int, std::string>, Region> regions_;
     DeviceBuffer state_buffer_;

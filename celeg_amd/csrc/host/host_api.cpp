@@ -94,6 +94,9 @@ Json call(HostObject& o, const std::string& method, const Json& a) {
         if (method == "covers") return Json(c.covers(static_cast<int>(a[0].as_int()), static_cast<int>(a[1].as_int()), static_cast<int>(a[2].as_int())));
         if (method == "pages_needed") return Json::array_of(c.pages_needed(static_cast<int>(a[0].as_int()), static_cast<int>(a[1].as_int()), static_cast<int>(a[2].as_int())));
         if (method == "check") { c.check(); return Json(true); }
+        if (method == "fork") return Json(c.fork(static_cast<int>(a[0].as_int()), static_cast<int>(a[1].as_int())));
+        if (method == "truncate") { c.truncate(static_cast<int>(a[0].as_int()), static_cast<int>(a[1].as_int())); return Json(true); }
+        if (method == "holds") return Json(c.holds(static_cast<int>(a[0].as_int()), static_cast<int>(a[1].as_int()), static_cast<int>(a[2].as_int())));
         if (method == "pages_held") {
             Json out = Json::array();
             for (const auto& g : c.pages_held(static_cast<int>(a[0].as_int()))) out.push(Json::array_of(g));

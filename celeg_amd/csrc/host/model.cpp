@@ -8,6 +8,8 @@
 #include <cstdlib>
 #include <set>
 
+#include "branch.hpp"
+
 namespace celeg {
 
 // ---------------------------------------------------------------------------- the model
@@ -180,6 +182,8 @@ void Model::load(const WeightMap& tensors, Runtime& rt) {
 }
 
 void Model::bind_cache(const CacheManager& cache) {
+    takes_trees_ = cache.layout.states.empty();
+    for (const auto& block : blocks_) takes_trees_ = takes_trees_ && block->mixer().takes_trees();
     caches_.clear();
     embedding_cache_ = cache.layer_cache(CacheLayout::EMBEDDING);
     for (size_t i = 0; i < spec.order.size(); ++i) caches_.push_back(cache.layer_cache(static_cast<int>(i)));
@@ -451,6 +455,8 @@ void ModelRunner::begin_step(const StepBatch& batch) {
 
 Tensor ModelRunner::step(const std::vector<StepEntry>& entries) {
     validate(entries);
+    for (const StepEntry& e : entries)
+        if (!e.parents.empty()) return step_of_trees(entries);
     if (graph_applies(entries)) return step_from_graph(entries);
     if (portion_graph_applies(entries)) return step_from_portion_graph(entries);
     auto updates = drain_updates(std::vector<int>(static_cast<size_t>(cache.n_groups()), update_room_));
@@ -465,6 +471,94 @@ Tensor ModelRunner::step(const std::vector<StepEntry>& entries) {
     if (rt.phases) rt.phases->end(batch.n_tokens);
     ++steps_run;
     return logits;
+}
+
+// A step in which tokens branch.  Their keys and values lie one after the other from the entry's start on, in the order given,
+// and they are rotated by start + depth.  Entries without parents are trees of one branch.
+Tensor ModelRunner::step_of_trees(const std::vector<StepEntry>& entries) {
+    if (!model.takes_trees()) throw StepError("step: this model has mixers or state that trees of drafted tokens cannot go through");
+    size_t most = 0;
+    for (const StepEntry& e : entries) {
+        most = std::max(most, e.tokens.size());
+        if (!e.parents.empty() && e.parents.size() != e.tokens.size()) throw StepError("step: one parent a token is needed");
+        for (size_t i = 0; i < e.parents.size(); ++i)
+            if (e.parents[i] < -1 || e.parents[i] >= static_cast<int>(i))
+                throw StepError("step: parent " + std::to_string(e.parents[i]) + " of token " + std::to_string(i) + " is not before it");
+    }
+    if (most > static_cast<size_t>(TreeAttention::MAX_NODES) || most * entries.size() > 65535)
+        throw StepError("step: trees of up to " + std::to_string(TreeAttention::MAX_NODES) + " tokens, up to 65,535 entries times the largest");
+    auto updates = drain_updates(std::vector<int>(static_cast<size_t>(cache.n_groups()), update_room_));
+    BuildOptions options;
+    options.null_slot = cache.null_slot;
+    StepBatch batch = build(entries, updates, options);
+    // positions and parents, in the order of the batch's rows
+    const size_t T = static_cast<size_t>(batch.n_tokens);
+    std::vector<int> rows(2 * T);
+    for (size_t j = 0; j < entries.size(); ++j) {
+        const StepEntry& e = entries[static_cast<size_t>(batch.entry_order[j])];
+        const size_t first = static_cast<size_t>(batch.host_cu_seqlens[j]);
+        for (size_t i = 0; i < e.tokens.size(); ++i) {
+            const int parent = e.parents.empty() ? static_cast<int>(i) - 1 : e.parents[i];
+            rows[first + i] = parent < 0 ? e.start_pos : rows[first + static_cast<size_t>(parent)] + 1;
+            rows[T + first + i] = parent;
+        }
+    }
+    int* staged = static_cast<int*>(rt.ws.raw("tree_rows", 2 * static_cast<size_t>(max_batched_tokens) * sizeof(int)));
+    CELEG_HIP(hipMemcpyAsync(staged, rows.data(), rows.size() * sizeof(int), hipMemcpyHostToDevice, rt.stream));
+    CELEG_HIP(hipStreamSynchronize(rt.stream));        // (the host vector goes away)
+    batch.tree_places = batch.positions;
+    batch.positions = staged;
+    batch.tree_parents = staged + T;
+    batch.max_tree_nodes = static_cast<int>(most);
+    batch.decode_only = false;
+    batch.single_rows = 0;
+    if (rt.phases) rt.phases->begin();
+    begin_step(batch);
+    rt.mark("step metadata");
+    last_batch_ = batch;
+    Tensor logits = model.forward(batch, rt);
+    if (rt.phases) rt.phases->end(batch.n_tokens);
+    ++steps_run;
+    return logits;
+}
+
+void ModelRunner::keep(int slot, int start, const std::vector<int>& places) {
+    if (!cache.layout.states.empty()) throw StepError("keep: the model keeps state, which cannot go back");
+    const int n = static_cast<int>(places.size());
+    if (start < 0) throw StepError("keep: start must not be negative");
+    for (int i = 0; i < n; ++i)
+        if (places[static_cast<size_t>(i)] < (i ? places[static_cast<size_t>(i) - 1] + 1 : start))
+            throw StepError("keep: the places must rise, from start on");
+    if (n && places.back() >= cache.tokens(slot))
+        throw StepError("keep: slot " + std::to_string(slot) + " has no token at place " + std::to_string(places.back()));
+    for (int i = 0; i < n; ++i)
+        if (!cache.holds(slot, places[static_cast<size_t>(i)], 1) || !cache.holds(slot, start + i, 1))
+            throw StepError("keep: slot " + std::to_string(slot) + " holds no page for place " + std::to_string(places[static_cast<size_t>(i)]) +
+                            " or " + std::to_string(start + i));
+    // (those that stand where they should already stay there)
+    int first = 0;
+    while (first < n && places[static_cast<size_t>(first)] == start + first) ++first;
+    if (first < n) {
+        if (!cache.unshare(slot, start + first, n - first)) throw StepError("keep: no free page for what is shared with another request");
+        // the device's block tables as the host's are
+        auto updates = cache.drain_table_updates();
+        for (size_t g = 0; g < updates.size(); ++g)
+            if (!updates[g].empty()) ship_table_updates(static_cast<int>(g), updates[g]);
+        std::vector<int> lists{slot, 0, n - first, start + first};
+        lists.insert(lists.end(), places.begin() + first, places.end());
+        int* staged = static_cast<int*>(rt.ws.raw("keep_lists", (4 + static_cast<size_t>(cache.max_context)) * sizeof(int)));
+        CELEG_HIP(hipMemcpyAsync(staged, lists.data(), lists.size() * sizeof(int), hipMemcpyHostToDevice, rt.stream));
+        MoveTokens move;
+        move.requests = 1;
+        move.n_places = n - first;
+        move.src_slots = move.dst_slots = staged;
+        move.offsets = staged + 1;
+        move.dst_starts = staged + 3;
+        move.places = staged + 4;
+        for (int g = 0; g < cache.n_groups(); ++g) move_tokens(move, cache.group_view(g), rt.stream);
+        CELEG_HIP(hipStreamSynchronize(rt.stream));
+    }
+    cache.truncate(slot, start + n);
 }
 
 // A step in which every request brings one token and wants its logits is bound by its number

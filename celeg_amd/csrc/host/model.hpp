@@ -35,6 +35,8 @@ public:
     // tensors: checkpoint name -> device tensor, already checked and converted
     void load(const WeightMap& tensors, Runtime& rt);
     void bind_cache(const CacheManager& cache);
+    // whether a step's entries may be trees: no state that a row leaves for the next one, and every mixer takes them
+    bool takes_trees() const { return takes_trees_; }
     // Runs the rows of `batch` through every entry of the run order and returns 32-bit logits
     // [batch.n_logit_rows, vocab] (a workspace buffer: it holds until the next step).
     Tensor forward(const StepBatch& batch, Runtime& rt);
@@ -55,7 +57,7 @@ private:
     std::unique_ptr<Head> head_;
     std::vector<LayerCache> caches_;
     LayerCache embedding_cache_;
-    bool bound_ = false, graph_safe_ = false;
+    bool bound_ = false, graph_safe_ = false, takes_trees_ = false;
 };
 
 // The step function: runs one batch of (request, its next tokens) through the model, from the
@@ -75,6 +77,10 @@ public:
     // Logits, 32-bit [number of wanted places, vocab] on the device, in the order of the entries
     // and of each entry's want.  The buffer is reused: it holds until the next step.
     Tensor step(const std::vector<StepEntry>& entries);
+    // Of a request's tokens from place `start` on, those at `places` (rising) stay and come to stand from `start` on; the others are
+    // forgotten and their pages given back.  What an accepted path of a tree is, or the kept tokens of a context (the keys
+    // keep the positions they were rotated by).  Refused where the model keeps state beside keys and values: it cannot go back.
+    void keep(int slot, int start, const std::vector<int>& places);
 
     Model& model;
     CacheManager& cache;
@@ -105,6 +111,7 @@ private:
     bool graph_applies(const std::vector<StepEntry>& entries) const;
     int context_bound(const std::vector<StepEntry>& entries, int bucket) const;
     std::map<int, std::vector<int>> short_contexts_;      // by the bucket of a recorded step
+    Tensor step_of_trees(const std::vector<StepEntry>& entries);
     Tensor step_from_graph(const std::vector<StepEntry>& entries);
     Captured& capture(int bucket, const std::vector<int>& caps, int bound);
     Captured& record(std::pair<int, int> key, const StepBatch& batch);

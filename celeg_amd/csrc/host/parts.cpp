@@ -10,6 +10,7 @@
 #include <cmath>
 #include <mutex>
 
+#include "branch.hpp"
 #include "kernels.hpp"
 
 namespace celeg {
@@ -419,6 +420,7 @@ public:
     }
     // h += mixer(norm(h)) with the norm folded into the q/k/v product and the residual addition
     // into the output product
+    bool takes_trees() const override { return head_dim_ <= TreeAttention::MAX_HEAD_DIM; }
     bool forward_fused(const Tensor& h, const Norm::Foldable& norm, const StepBatch& batch, const LayerCache& cache,
                        Runtime& rt) override {
         const long long qw = static_cast<long long>(heads_) * head_dim_;
@@ -452,7 +454,7 @@ private:
         bool finished = false;      // norm, rotation and cache write made by the product's own kernel
         if (writes) {
             Tensor qkv = rt.ws.buf("attn_qkv", rt.dtype, {T, qw + 2 * kvw});
-            if (norm && fused::qkv_tail_ok(rt, static_cast<int>(T), width_) && T == batch.n_tokens &&
+            if (norm && !batch.tree_places && fused::qkv_tail_ok(rt, static_cast<int>(T), width_) && T == batch.n_tokens &&
                 rt.ops.tiled_qkv_ok(head_dim_, inv_freq, tables.rotary_dim, tables.pairing, *cache.kv)) {
                 QkvTail tail;
                 tail.heads = heads_;
@@ -479,6 +481,43 @@ private:
             project(w_q_, q);
         }
         Tensor attended = rt.ws.buf("attn_out", rt.dtype, {T, qw});
+        if (batch.tree_places) {
+            // nodes of trees: turned by their positions, then put to their places
+            auto turn = [&](const Tensor& x, const std::shared_ptr<DeviceTensor>& weight, int heads) {
+                rt.ops.qk_norm_rope_store(x, nullptr, nullptr, weight ? &weight->view : nullptr, nullptr, eps_, inv_freq, tables.rotary_dim,
+                                          tables.pairing, heads, kv_heads_, head_dim_, batch, *cache.kv);
+            };
+            turn(q, q_norm_, heads_);
+            if (writes) {
+                turn(k, k_norm_, kv_heads_);
+                StepBatch at;
+                at.n_tokens = batch.n_tokens;
+                at.positions = batch.tree_places;
+                at.token_slot = batch.token_slot;
+                rt.ops.qk_norm_rope_store(q, &k, &v, nullptr, nullptr, eps_, nullptr, 0, 0, heads_, kv_heads_, head_dim_, at, *cache.kv);
+            }
+            TreeAttention a;
+            a.q = q.data;
+            a.q_stride = q.row_stride();
+            a.out = attended.data;
+            a.rows = batch.n_tokens;
+            a.heads = heads_;
+            a.requests = batch.n_seqs;
+            a.slots = batch.seq_slot;
+            a.starts = batch.seq_start;
+            a.offsets = batch.cu_seqlens;
+            a.parents = batch.tree_parents;
+            a.scale = scale_;
+            a.window = window_ ? *window_ : 0;
+            a.max_nodes = batch.max_tree_nodes;
+            a.max_context = batch.context_hint();
+            // (room by powers of two: a workspace that grows with every longer context would keep all its former selves)
+            const size_t needed = tree_attention_workspace(a, *cache.kv);
+            size_t bytes = needed ? size_t(1) << 16 : 0;
+            while (bytes < needed) bytes *= 2;
+            tree_attention(a, *cache.kv, bytes ? rt.ws.raw("tree_parts", bytes) : nullptr, bytes, rt.stream);
+            return attended;
+        }
         // a decode-only step: the attention kernel prepares and writes the step's own keys and values
         if (!finished && writes && T == batch.n_tokens &&
             rt.ops.attention_fresh_ok(heads_, head_dim_, inv_freq, tables.rotary_dim, tables.pairing, batch, *cache.kv, rt.dtype)) {

@@ -123,6 +123,8 @@ public:
     // h += mixer(norm(h)); false (nothing done) if this step cannot take the fused path
     virtual bool forward_fused(const Tensor& h, const Norm::Foldable& norm, const StepBatch& batch,
                                const LayerCache& cache, Runtime& rt) { return false; }
+    // whether a step's entries may be trees of drafted tokens (StepBatch::tree_places): rows that do not follow one another
+    virtual bool takes_trees() const { return false; }
 };
 
 class FeedForward : public Part {

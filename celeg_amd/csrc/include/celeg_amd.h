@@ -164,6 +164,29 @@ const char* celeg_model_cache_state(celeg_model* model);
 celeg_status celeg_model_step(celeg_model* model, int32_t n_entries, const int32_t* slot, const int32_t* start_pos,
                               const int32_t* n_tokens, const int32_t* tokens, const int32_t* n_want,
                               const int32_t* want, float* logits, size_t capacity);
+/* The same for entries that are trees of drafted tokens: parents holds for every token the index of its parent among the entry's
+ * tokens, lower than its own, or -1 (it follows the start itself); null: no trees.  A token sees what lies before the
+ * start, its ancestors and itself; it stands at start_pos + its depth, its key and value lie at start_pos + its index
+ * until celeg_model_keep brings an accepted path together.  Up to 256 tokens an entry.  For models whose mixers are all
+ * softmax attention and that keep no other state (celeg_model_describe: "takes_trees"); others refuse it. */
+celeg_status celeg_model_step_tree(celeg_model* model, int32_t n_entries, const int32_t* slot, const int32_t* start_pos,
+                                   const int32_t* n_tokens, const int32_t* tokens, const int32_t* parents, const int32_t* n_want,
+                                   const int32_t* want, float* logits, size_t capacity);
+/* A step of which the logits stay on the device: what they say about tokens comes back (celeg_token_logprobs), for every
+ * wanted place: of per_row (up to 8) targets [wanted, per_row] the log probabilities and ranks, the entropy [wanted], and the
+ * `top` (up to 128) best tokens with their log probabilities [wanted, top].  All in host memory. */
+celeg_status celeg_model_step_logprobs(celeg_model* model, int32_t n_entries, const int32_t* slot, const int32_t* start_pos,
+                                       const int32_t* n_tokens, const int32_t* tokens, const int32_t* parents, const int32_t* n_want,
+                                       const int32_t* want, const int32_t* targets, int32_t per_row, int32_t top, float* logprobs,
+                                       int32_t* ranks, float* entropy, int32_t* top_ids, float* top_logprobs);
+/* A slot for a request that goes on from the first `length` tokens of another (of those celeg_model_prepare has given it pages
+ * for), its state beside keys and values as it stands.  Pages are shared; celeg_model_prepare gives whoever writes to a shared one
+ * a copy of its own (both have to call it before their next step).  *new_slot -1: every slot is taken. */
+celeg_status celeg_model_fork_slot(celeg_model* model, int32_t slot, int32_t length, int32_t* new_slot);
+/* Of a slot's tokens from place `start` on, those at the n `places` (rising) stay and come to stand at start, start + 1, ..; the rest is
+ * forgotten, and pages that hold nothing any more are given back.  n 0: the tokens before start alone stay.  Keys keep the
+ * positions they were turned by: the accepted path of a tree stands where it should.  Refused for models that keep state. */
+celeg_status celeg_model_keep(celeg_model* model, int32_t slot, int32_t start, const int32_t* places, int32_t n);
 /* ---- one request at a time on a model of its own (the reference's celeg_model_prefill / decode /
  * copy_logits / get_metrics, include/celeg/api.h:158-164, src/api/model.cpp:32-77): prefill starts a new
  * sequence with a prompt (what the model held of an earlier one is given back); decode chooses the next

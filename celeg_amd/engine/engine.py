@@ -11,7 +11,7 @@ from __future__ import annotations
 
 import enum
 from dataclasses import dataclass, field
-from typing import Any, Dict, List, Optional, Sequence, Tuple
+from typing import Any, Dict, List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -47,6 +47,18 @@ class StepEntry:
     start_pos: int            # position of tokens[0] in the request's sequence
     tokens: Sequence[int]
     want: Sequence[int] = ()  # indices into ``tokens`` whose logits are wanted
+    # drafted tokens that branch: of each token the index of its parent, -1: it follows the start (empty: every token follows
+    # the one before it); for models that ``take_trees``
+    parents: Sequence[int] = ()
+
+
+class StepLogprobs(NamedTuple):
+    """What a step's logits say about tokens, a row for every wanted place (on the host)."""
+    logprobs: torch.Tensor        # float32 [wanted, targets]
+    ranks: torch.Tensor           # int32, likewise: how many tokens stand ahead of the target
+    entropy: torch.Tensor         # float32 [wanted], nats
+    top_ids: torch.Tensor         # int32 [wanted, top]
+    top_logprobs: torch.Tensor    # float32 [wanted, top]
 
 
 class RequestStatus(enum.Enum):
@@ -108,6 +120,22 @@ class _CacheFacade:
     def prepare(self, slot: int, start_pos: int, n_new: int) -> bool:
         return self._m.prepare(slot, start_pos, n_new)
 
+    def fork(self, slot: int, length: int) -> Optional[int]:
+        """A slot that goes on from the first ``length`` tokens of another, with its state as it stands; the pages are shared
+        until ``prepare`` says that one of the two writes to one.  None: every slot is taken."""
+        try:
+            return self._m.fork_slot(slot, length)
+        except native.NativeError as err:
+            raise ValueError(str(err)) from None
+
+    def keep(self, slot: int, start: int, places: Sequence[int] = ()) -> None:
+        """Of the tokens from place ``start`` on, those at ``places`` (rising) stay, brought together from ``start`` on: the accepted
+        path of a tree, or the kept tokens of a context; the rest is forgotten.  ValueError for a model that keeps state."""
+        try:
+            self._m.keep(slot, start, places)
+        except native.NativeError as err:
+            raise ValueError(str(err)) from None
+
     def check(self) -> None:
         self._m.check_cache()
 
@@ -135,6 +163,14 @@ class _RunnerFacade:
         entries and of each entry's ``want``."""
         try:
             return torch.from_numpy(self._m.step(entries))
+        except native.NativeError as err:
+            raise ValueError(str(err)) from None
+
+    def logprobs(self, entries: Sequence[StepEntry], targets=None, top: int = 0) -> StepLogprobs:
+        """A step whose logits stay on the device; ``targets`` [wanted places, up to 8]: token ids whose log probabilities and ranks
+        are asked for, ``top``: how many of the best tokens (up to 128)."""
+        try:
+            return StepLogprobs(*(torch.from_numpy(x) for x in self._m.step_logprobs(entries, targets, top)))
         except native.NativeError as err:
             raise ValueError(str(err)) from None
 
@@ -166,6 +202,39 @@ class LoadedModel:
         self.runner = _RunnerFacade(model)
         self.dtype = info["dtype"]
         self.graph_safe = info["graph_safe"]
+
+    @property
+    def takes_trees(self) -> bool:
+        """Whether a step's entries may be trees of drafted tokens (``StepEntry.parents``)."""
+        return bool(self.native.info["takes_trees"])
+
+    def score(self, tokens: Sequence[int], top: int = 0, portion: Optional[int] = None) -> StepLogprobs:
+        """A sequence judged token by token: row i says what the model expected behind ``tokens[:i + 1]``, its target being
+        ``tokens[i + 1]`` (one row fewer than tokens), with the ``top`` best tokens there.  Takes a slot of the
+        cache for the time of the call; in portions of at most ``portion`` tokens (the step's largest)."""
+        tokens = [int(t) for t in tokens]
+        portion = min(portion or self.runner.max_batched_tokens, self.runner.max_batched_tokens)
+        slot = self.cache.open()
+        if slot is None:
+            raise ValueError("score: every slot of the cache is taken")
+        try:
+            parts = []
+            for at in range(0, max(len(tokens) - 1, 0), portion):
+                part = tokens[at:min(at + portion, len(tokens) - 1)]
+                try:
+                    prepared = self.cache.prepare(slot, at, len(part))
+                except native.NativeError as err:
+                    raise ValueError(str(err)) from None
+                if not prepared:
+                    raise ValueError("score: too few free pages")
+                targets = [[t] for t in tokens[at + 1:at + 1 + len(part)]]
+                parts.append(self.runner.logprobs([StepEntry(slot, at, part, range(len(part)))], targets, top))
+        finally:
+            self.cache.close(slot)
+        if not parts:
+            return StepLogprobs(torch.empty(0, 1), torch.empty(0, 1, dtype=torch.int32), torch.empty(0), torch.empty(0, top, dtype=torch.int32),
+                                torch.empty(0, top))
+        return StepLogprobs(*(torch.cat(of) for of in zip(*parts)))
 
     def set_knob(self, name: str, value) -> None:
         self.native.set_knob(name, value)

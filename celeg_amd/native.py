@@ -170,6 +170,12 @@ def lib() -> ctypes.CDLL:
     sig("celeg_model_cache_state", c_char_p, c_void_p)
     sig("celeg_model_step", c_int, c_void_p, c_int32, P(c_int32), P(c_int32), P(c_int32), P(c_int32), P(c_int32),
         P(c_int32), c_void_p, c_size_t)
+    sig("celeg_model_step_tree", c_int, c_void_p, c_int32, P(c_int32), P(c_int32), P(c_int32), P(c_int32), P(c_int32), P(c_int32),
+        P(c_int32), c_void_p, c_size_t)
+    sig("celeg_model_step_logprobs", c_int, c_void_p, c_int32, P(c_int32), P(c_int32), P(c_int32), P(c_int32), P(c_int32), P(c_int32),
+        P(c_int32), c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p)
+    sig("celeg_model_fork_slot", c_int, c_void_p, c_int32, c_int32, P(c_int32))
+    sig("celeg_model_keep", c_int, c_void_p, c_int32, c_int32, P(c_int32), c_int32)
     sig("celeg_model_set_knob", c_int, c_void_p, c_char_p, c_int32)
     sig("celeg_model_knobs", c_char_p, c_void_p)
     sig("celeg_model_stream", c_void_p, c_void_p)
@@ -299,6 +305,20 @@ def device_index(device) -> int:
 
 
 # ------------------------------------------------------------------ the step function alone
+def _step_lists(entries):
+    """The entries of a step as the C interface takes them.  With a tree among them (``parents``), the others' tokens follow
+    one another."""
+    parents = None
+    if any(getattr(e, "parents", None) for e in entries):
+        listed = [list(e.parents) if getattr(e, "parents", None) else list(range(-1, len(e.tokens) - 1)) for e in entries]
+        if any(len(p) != len(e.tokens) for p, e in zip(listed, entries)):
+            raise NativeArgumentError("one parent a token is needed")
+        parents = _ints([int(p) for of in listed for p in of])
+    return (_ints([int(e.slot) for e in entries]), _ints([int(e.start_pos) for e in entries]), _ints([len(e.tokens) for e in entries]),
+            _ints([int(t) for e in entries for t in e.tokens]), parents, _ints([len(e.want) for e in entries]),
+            _ints([int(w) for e in entries for w in e.want]), sum(len(e.want) for e in entries))
+
+
 class NativeModel:
     """A loaded model with its cache manager and runner (``celeg_model``)."""
 
@@ -346,19 +366,36 @@ class NativeModel:
         return json.loads(_text(lib().celeg_model_cache_state(self.handle)))
 
     def step(self, entries) -> np.ndarray:
-        """``entries``: objects with slot, start_pos, tokens, want.  Returns float32
+        """``entries``: objects with slot, start_pos, tokens, want and, for trees of drafted tokens, parents.  Returns float32
         [wanted, logit width]."""
-        slots = _ints([int(e.slot) for e in entries])
-        starts = _ints([int(e.start_pos) for e in entries])
-        counts = _ints([len(e.tokens) for e in entries])
-        tokens = _ints([int(t) for e in entries for t in e.tokens])
-        n_want = _ints([len(e.want) for e in entries])
-        want = _ints([int(w) for e in entries for w in e.want])
-        wanted = sum(len(e.want) for e in entries)
+        slots, starts, counts, tokens, parents, n_want, want, wanted = _step_lists(entries)
         out = np.empty((wanted, self.logit_width), dtype=np.float32)
-        check(lib().celeg_model_step(self.handle, len(entries), slots, starts, counts, tokens, n_want, want,
-                                     out.ctypes.data_as(c_void_p), out.size))
+        check(lib().celeg_model_step_tree(self.handle, len(entries), slots, starts, counts, tokens, parents, n_want, want,
+                                          out.ctypes.data_as(c_void_p), out.size))
         return out
+
+    def step_logprobs(self, entries, targets, top: int = 0):
+        """``targets``: int32 [wanted, up to 8] (None: none).  Returns (logprobs, ranks, entropy, top_ids, top_logprobs)."""
+        slots, starts, counts, tokens, parents, n_want, want, wanted = _step_lists(entries)
+        targets = np.zeros((wanted, 0), np.int32) if targets is None else np.ascontiguousarray(targets, np.int32)
+        if targets.ndim != 2 or targets.shape[0] != wanted:
+            raise NativeArgumentError(f"targets must be [wanted places, n]: {wanted} rows, not {targets.shape}")
+        n, top = targets.shape[1], int(top)
+        if not 0 <= top <= 128 or n > 8:
+            raise NativeArgumentError("up to 128 best tokens and 8 targets a place")
+        out = (np.empty((wanted, n), np.float32), np.empty((wanted, n), np.int32), np.empty(wanted, np.float32),
+               np.empty((wanted, top), np.int32), np.empty((wanted, top), np.float32))
+        check(lib().celeg_model_step_logprobs(self.handle, len(entries), slots, starts, counts, tokens, parents, n_want, want,
+                                              targets.ctypes.data_as(c_void_p), n, top, *(o.ctypes.data_as(c_void_p) for o in out)))
+        return out
+
+    def fork_slot(self, slot: int, length: int) -> Optional[int]:
+        new = c_int32()
+        check(lib().celeg_model_fork_slot(self.handle, slot, length, ctypes.byref(new)))
+        return None if new.value < 0 else new.value
+
+    def keep(self, slot: int, start: int, places: Sequence[int]) -> None:
+        check(lib().celeg_model_keep(self.handle, slot, start, _ints([int(p) for p in places]), len(places)))
 
     def set_knob(self, name: str, value) -> None:
         check(lib().celeg_model_set_knob(self.handle, name.encode(), int(value)))
