@@ -8,8 +8,12 @@
 //
 // What bounds it is the one read of the logits.  A workgroup of 256 threads takes a part of a row into its registers (up to
 // 64 logits a thread), and finds there in turn the maximum, the sums, the tokens' ranks and the part's best: four such
-// workgroups share a compute unit, so that one's arithmetic runs while another's loads are on their way.  Few rows are cut into
-// more parts, so that all compute units take part; a second kernel, a workgroup a row, joins the parts.
+// workgroups share a compute unit, so that one's arithmetic runs while another's loads are on their way; a second kernel, a
+// workgroup a row, joins the parts.  2,048 rows of 65,536 32-bit logits, 5 best: 104 us (5.2 TB/s, as a large copy); of bfloat16 80 us,
+// bound by the vector instructions (an exponential is four of the about 20 a logit).  Up to 256 rows, one a compute unit, have
+// nothing to overlap with: there a workgroup of 1,024 threads takes a whole row of up to 65,536 logits, and nothing is joined (one row 11.0
+// us where parts and their join take 12.0, and a launch and a workspace less for the host; 64 rows, 20 best 12.1 and 14.7; 128 best
+// of one row 25 and 140).
 //
 // The best of a part: the top-th largest of the maxima of 64 (256) groups of threads is not above the top-th largest logit,
 // so that the logits not below it hold all that is sought and little more; they are collected and counted against one another.
@@ -28,6 +32,7 @@ typedef float lp_f4 __attribute__((ext_vector_type(4)));
 typedef unsigned int lp_u4 __attribute__((ext_vector_type(4)));
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr float LP_FITS = 1e38f;          // below it a logit times log2(e) is a number
 
 // 16 bytes of logits as they lie in memory
 template <typename T> struct LogitGroup;
@@ -70,12 +75,26 @@ __device__ __forceinline__ float best_logit(unsigned long long packed) {
     return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
 }
 
-__device__ __forceinline__ float logprob_of(float x, float m, float log2_sum) { return (x - m) - log2_sum * LN2; }
+// x's distance from the largest, in powers of two, as the sums take it
+__device__ __forceinline__ float logit_distance(float x, float m) { return fabsf(m) < LP_FITS ? fmaf(x, LOG2E, -(m * LOG2E)) : (x - m) * LOG2E; }
+
+__device__ __forceinline__ float logprob_of(float x, float m, float log2_sum) {
+    const float d = logit_distance(x, m);
+    return d == -INFINITY ? (x - m) - log2_sum * LN2 : (d - log2_sum) * LN2;       // (what is far below may fit in nats alone)
+}
 
 // Of n packed logits in `list` (all different), the `top` largest in falling order: put(place, packed).  All threads call it.
-template <typename F>
+// The same of a part's largest, as the part has it: its sums are against the rounded product.
+__device__ __forceinline__ float part_distance(float part, float m) {
+    if (!(fabsf(part) < LP_FITS && fabsf(m) < LP_FITS)) return (part - m) * LOG2E;
+    float of_part = part * LOG2E;
+    asm volatile("" : "+v"(of_part));        // (rounded, as the part's sums have it: not taken into the subtraction)
+    return of_part - m * LOG2E;
+}
+
+template <int THREADS, typename F>
 __device__ __forceinline__ void sorted_best(const unsigned long long* list, int n, int top, F put) {
-    for (int i = threadIdx.x; i < n; i += LP_THREADS) {
+    for (int i = threadIdx.x; i < n; i += THREADS) {
         const unsigned long long mine = list[i];
         int ahead = 0;
         for (int j = 0; j < n; ++j) ahead += list[j] > mine;
@@ -87,20 +106,23 @@ __device__ __forceinline__ void sorted_best(const unsigned long long* list, int 
 // Too many logits lie at or above the bound for the list (thousands of equal ones, or a bound of -inf where a vocabulary is
 // masked down to a few tokens): exactly the `top` best of columns c0 .. c1 - 1 go to the list.  The logits are read again for
 // every halving; all threads call it.  (No NaN among them.)
-template <typename T>
+template <typename T, int THREADS>
 __device__ __noinline__ int best_by_halving(const T* __restrict__ x, int c0, int c1, int top, float bound, float high,
                                             unsigned long long* list, int* counts, int* count) {
+    constexpr int WAVES = THREADS / 64;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int turn = 0;
     auto count_of = [&](auto take) {
         int n = 0;
-        for (int c = c0 + tid; c < c1; c += LP_THREADS) n += take(order_key(to_float(x[c]) + 0.0f), c);
+        for (int c = c0 + tid; c < c1; c += THREADS) n += take(order_key(to_float(x[c]) + 0.0f), c);
         const float of_wave = wave_sum(static_cast<float>(n));
         turn ^= 1;                       // (the other half of counts may still be read)
-        if (lane == 0) counts[turn * LP_WAVES + wave] = static_cast<int>(of_wave);
+        if (lane == 0) counts[turn * WAVES + wave] = static_cast<int>(of_wave);
         __syncthreads();
-        const int* of = counts + turn * LP_WAVES;
-        return of[0] + of[1] + of[2] + of[3];
+        const int* of = counts + turn * WAVES;
+        int all = 0;
+        for (int i = 0; i < WAVES; ++i) all += of[i];
+        return all;
     };
     // the largest key that `wanted` logits are not below
     const int wanted = min(top, c1 - c0);
@@ -121,7 +143,7 @@ __device__ __noinline__ int best_by_halving(const T* __restrict__ x, int c0, int
     __syncthreads();
     if (tid == 0) *count = 0;
     __syncthreads();
-    for (int c = c0 + tid; c < c1; c += LP_THREADS) {
+    for (int c = c0 + tid; c < c1; c += THREADS) {
         const float v = to_float(x[c]);
         const uint32_t k = order_key(v + 0.0f);
         if (k > key || (k == key && c <= last)) {
@@ -135,18 +157,18 @@ __device__ __noinline__ int best_by_halving(const T* __restrict__ x, int c0, int
 
 // A thread holds GROUPS groups of 16 bytes, and one logit more where the part begins or ends off a boundary of 16 bytes.  What
 // it holds beyond the part is a NaN: no comparison and no sum takes it.
-template <typename T, int GROUPS>
-__global__ __launch_bounds__(LP_THREADS, 4) void logprobs_part_kernel(
+template <typename T, int GROUPS, int THREADS>
+__global__ __launch_bounds__(THREADS, 1024 / THREADS) void logprobs_part_kernel(
     const T* __restrict__ logits, long long row_stride, const int* __restrict__ tokens, int vocab, int per_row, int top, int parts,
     int part_size, const LogprobParts left, const LogprobOut out) {
     using Group = LogitGroup<T>;
-    constexpr int N = Group::N;
-    __shared__ float wave_of[LP_WAVES][2 + LP_MAX_TOKENS];
-    __shared__ float wave_high[LP_WAVES];
-    __shared__ int wave_bad[LP_WAVES];
-    __shared__ __align__(16) float maxima[LP_THREADS];
-    __shared__ float bounds[LP_WAVES];
-    __shared__ int n_groups, count, counts[2 * LP_WAVES];
+    constexpr int N = Group::N, WAVES = THREADS / 64;
+    __shared__ float wave_of[WAVES][2 + LP_MAX_TOKENS];
+    __shared__ float wave_high[WAVES];
+    __shared__ int wave_bad[WAVES];
+    __shared__ __align__(16) float maxima[256];
+    __shared__ float bounds[4];
+    __shared__ int n_groups, count, counts[2 * WAVES];
     __shared__ Group hit[LP_GROUPS];
     __shared__ int hit_at[LP_GROUPS];
     __shared__ unsigned long long list[LP_LIST];
@@ -162,7 +184,7 @@ __global__ __launch_bounds__(LP_THREADS, 4) void logprobs_part_kernel(
     if (whole > 0) {
         const decltype(g[0].v)* from = reinterpret_cast<const decltype(g[0].v)*>(x + a0);
 #pragma unroll
-        for (int j = 0; j < GROUPS; ++j) g[j].v = from[min(tid + j * LP_THREADS, whole - 1)];
+        for (int j = 0; j < GROUPS; ++j) g[j].v = from[min(tid + j * THREADS, whole - 1)];
     } else {
 #pragma unroll
         for (int j = 0; j < GROUPS; ++j) g[j].none();
@@ -182,10 +204,10 @@ __global__ __launch_bounds__(LP_THREADS, 4) void logprobs_part_kernel(
         n_groups = 0;
         count = 0;
     }
-    if (whole < GROUPS * LP_THREADS) {
+    if (whole < GROUPS * THREADS) {
 #pragma unroll
         for (int j = 0; j < GROUPS; ++j)
-            if (tid + j * LP_THREADS >= whole) g[j].none();
+            if (tid + j * THREADS >= whole) g[j].none();
     }
     // ---- the maximum
     float high = fmaxf(-INFINITY, extra);
@@ -199,29 +221,46 @@ __global__ __launch_bounds__(LP_THREADS, 4) void logprobs_part_kernel(
             high = fmaxf(high, v);
             of_group |= v != v;
         }
-        bad |= of_group && tid + j * LP_THREADS < whole;
+        bad |= of_group && tid + j * THREADS < whole;
     }
     const bool any_bad = __ballot(bad) != 0ull;
     const float wave_max_value = wave_max(high);
-    // (the maxima of 4 lanes each where 64 are well more than are sought)
+    // 256 maxima, or 64 (of four times as many threads) where those are well more than are sought
     const bool few = top <= 40;
+    float of_some = high;
+    if (THREADS > 256) {
+        of_some = fmaxf(of_some, lane_move<LANES_XOR_1>(of_some));
+        of_some = fmaxf(of_some, lane_move<LANES_XOR_2>(of_some));
+    }
     if (few) {
-        float of_four = fmaxf(high, lane_move<LANES_XOR_1>(high));
-        of_four = fmaxf(of_four, lane_move<LANES_XOR_2>(of_four));
-        if ((lane & 3) == 0) maxima[tid >> 2] = of_four;
-    } else {
-        maxima[tid] = high;
+        if (THREADS > 256) {
+            of_some = fmaxf(of_some, lane_move<LANES_ROTATE_8>(of_some));
+            of_some = fmaxf(of_some, lane_move<LANES_ROTATE_4>(of_some));
+            if ((lane & 15) == 0) maxima[tid >> 4] = of_some;
+        } else {
+            of_some = fmaxf(of_some, lane_move<LANES_XOR_1>(of_some));
+            of_some = fmaxf(of_some, lane_move<LANES_XOR_2>(of_some));
+            if ((lane & 3) == 0) maxima[tid >> 2] = of_some;
+        }
+    } else if (THREADS == 256 || (lane & 3) == 0) {
+        maxima[THREADS == 256 ? tid : tid >> 2] = of_some;
     }
     if (lane == 0) {
         wave_high[wave] = wave_max_value;
         wave_bad[wave] = any_bad;
     }
     __syncthreads();
-    high = fmaxf(fmaxf(wave_high[0], wave_high[1]), fmaxf(wave_high[2], wave_high[3]));
-    bad = (wave_bad[0] | wave_bad[1] | wave_bad[2] | wave_bad[3]) != 0;
+    high = wave_high[0];
+    int any = wave_bad[0];
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) {
+        high = fmaxf(high, wave_high[i]);
+        any |= wave_bad[i];
+    }
+    bad = any != 0;
     // ---- the bound for the best: the least of the maxima that fewer than `top` others lie above
-    if (top > 0 && tid < (few ? 64 : LP_THREADS)) {
-        const int n = few ? 64 : LP_THREADS;
+    if (top > 0 && tid < (few ? 64 : 256)) {
+        const int n = few ? 64 : 256;
         const float mine = maxima[tid];
         int above = 0;
         for (int j = 0; j < n; j += 4) {
@@ -232,21 +271,27 @@ __global__ __launch_bounds__(LP_THREADS, 4) void logprobs_part_kernel(
         const float least = -wave_max(above < top ? -mine : -INFINITY);
         if (lane == 0) bounds[wave] = least;
     }
-    // ---- the sums.  (The maximum is taken off first: a mask of the type's lowest value times log2(e) would be no number.)
-    // Below -2000 the exponential is 0 in any case, and 0 times -2000 is no NaN.
+    // ---- the sums, of d = x log2(e) - m log2(e).  Below -2000 the exponential is 0 in any case, and 0 times -2000 is no NaN.
+    // Where m log2(e) would not fit (a row of the type's lowest value), the maximum is taken off first.
     const float m = high == -INFINITY ? 0.f : high;
     float sum = 0.f, moment = 0.f;
-    auto add = [&](float v) {
-        const float d = fmaxf((v - m) * LOG2E, -2000.f);
+    auto add = [&](float d) {
+        d = fmaxf(d, -2000.f);
         const float p = __builtin_amdgcn_exp2f(d);
         sum += p;
         moment = fmaf(p, d, moment);
     };
+    if (fabsf(m) < LP_FITS) {
+        const float m2 = m * LOG2E;
 #pragma unroll
-    for (int j = 0; j < GROUPS; ++j)
+        for (int j = 0; j < GROUPS; ++j)
 #pragma unroll
-        for (int e = 0; e < N; ++e) add(g[j].get(e));
-    add(extra);
+            for (int e = 0; e < N; ++e) add(fmaf(g[j].get(e), LOG2E, -m2));
+        add(fmaf(extra, LOG2E, -m2));
+    } else {
+        // (from memory: such rows are rare, and a second loop over the registers would take more of them)
+        for (int c = c0 + tid; c < c1; c += THREADS) add((to_float(x[c]) - m) * LOG2E);
+    }
     sum = wave_sum(sum);
     moment = wave_sum(moment);
     if (lane == 0) {
@@ -259,23 +304,23 @@ __global__ __launch_bounds__(LP_THREADS, 4) void logprobs_part_kernel(
         const float v = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, at), i));
         int ahead = 0;
         if (v == -INFINITY) {                   // (nothing is below it: counted from memory)
-            for (int c = c0 + tid; c < c1; c += LP_THREADS) ahead += to_float(x[c]) > v || c < t;
+            for (int c = c0 + tid; c < c1; c += THREADS) ahead += to_float(x[c]) > v || c < t;
         } else {
             const float below = next_below(v);
             // before the token, "not below it" is "above the next number below it"
             const int before = t >= a0 ? (t - a0) / N : 0;
 #pragma unroll
             for (int j = 0; j < GROUPS; ++j) {
-                const float over = tid + j * LP_THREADS < before ? below : v;
+                const float over = tid + j * THREADS < before ? below : v;
 #pragma unroll
                 for (int e = 0; e < N; ++e) ahead += g[j].get(e) > over;
             }
             ahead += extra > v || (extra == v && edge < t);
             // the group that the token lies in
-            if (before < whole && tid == before % LP_THREADS)
+            if (before < whole && tid == before % THREADS)
                 for (int c = a0 + before * N; c < t; ++c) ahead += to_float(x[c]) == v;
         }
-        const float total = wave_sum(static_cast<float>(ahead));       // (at most 16,384: exact)
+        const float total = wave_sum(static_cast<float>(ahead));       // (at most 2^17: exact)
         if (lane == 0) wave_of[wave][2 + i] = total;
     }
     __syncthreads();
@@ -292,14 +337,14 @@ __global__ __launch_bounds__(LP_THREADS, 4) void logprobs_part_kernel(
                 const int place = atomicAdd(&n_groups, 1);
                 if (place < LP_GROUPS) {
                     hit[place] = g[j];
-                    hit_at[place] = a0 + (tid + j * LP_THREADS) * N;
+                    hit_at[place] = a0 + (tid + j * THREADS) * N;
                 }
             }
         }
         if (extra >= bound) list[atomicAdd(&count, 1)] = packed_logit(extra, edge);        // (up to 2N of them)
         __syncthreads();
         const int hits = min(n_groups, LP_GROUPS);
-        for (int i = tid; i < hits * N; i += LP_THREADS) {
+        for (int i = tid; i < hits * N; i += THREADS) {
             const float v = hit[i / N].get(i % N);
             if (v >= bound) {
                 const int place = atomicAdd(&count, 1);
@@ -308,19 +353,24 @@ __global__ __launch_bounds__(LP_THREADS, 4) void logprobs_part_kernel(
         }
         __syncthreads();
         have = count;
-        if (n_groups > LP_GROUPS || have > LP_LIST) have = best_by_halving(x, c0, c1, top, bound, high, list, counts, &count);
+        if (n_groups > LP_GROUPS || have > LP_LIST) have = best_by_halving<T, THREADS>(x, c0, c1, top, bound, high, list, counts, &count);
     }
-    sum = wave_of[0][0] + wave_of[1][0] + wave_of[2][0] + wave_of[3][0];
-    moment = wave_of[0][1] + wave_of[1][1] + wave_of[2][1] + wave_of[3][1];
+    auto of_all = [&](int i) {
+        float all = (wave_of[0][i] + wave_of[1][i]) + (wave_of[2][i] + wave_of[3][i]);
+#pragma unroll
+        for (int w = 4; w < WAVES; w += 4) all += (wave_of[w][i] + wave_of[w + 1][i]) + (wave_of[w + 2][i] + wave_of[w + 3][i]);
+        return all;
+    };
+    sum = of_all(0);
+    moment = of_all(1);
     if (parts > 1) {
         const size_t at_part = row * parts + part;
         if (tid == 0) left.stats[at_part] = make_float4(high, sum, moment, bad ? 1.f : 0.f);
         if (tid < per_row)
-            left.ranks[at_part * per_row + tid] =
-                static_cast<int>(wave_of[0][2 + tid] + wave_of[1][2 + tid] + wave_of[2][2 + tid] + wave_of[3][2 + tid]);
+            left.ranks[at_part * per_row + tid] = static_cast<int>(of_all(2 + tid));       // (at most 2^17: exact)
         unsigned long long* best = left.best + at_part * top;
-        for (int k = have + tid; k < top; k += LP_THREADS) best[k] = 0ull;
-        sorted_best(list, have, top, [&](int place, unsigned long long packed) { best[place] = packed; });
+        for (int k = have + tid; k < top; k += THREADS) best[k] = 0ull;
+        sorted_best<THREADS>(list, have, top, [&](int place, unsigned long long packed) { best[place] = packed; });
         return;
     }
     const bool none = bad || high == INFINITY || high == -INFINITY;
@@ -329,18 +379,18 @@ __global__ __launch_bounds__(LP_THREADS, 4) void logprobs_part_kernel(
     if (tid < per_row) {
         const int t = tokens[row * per_row + tid];
         const bool valid = t >= 0 && t < vocab;
-        const float total = wave_of[0][2 + tid] + wave_of[1][2 + tid] + wave_of[2][2 + tid] + wave_of[3][2 + tid];
+        const float total = of_all(2 + tid);
         out.logprobs[row * per_row + tid] = valid ? logprob_of(to_float(x[t]), m, log2_sum) : NAN;
         out.ranks[row * per_row + tid] = valid && !bad ? static_cast<int>(total) : -1;
     }
     if (bad) {
-        for (int k = tid; k < top; k += LP_THREADS) {
+        for (int k = tid; k < top; k += THREADS) {
             out.top_ids[row * top + k] = -1;
             out.top_logprobs[row * top + k] = NAN;
         }
         return;
     }
-    sorted_best(list, have, top, [&](int place, unsigned long long packed) {
+    sorted_best<THREADS>(list, have, top, [&](int place, unsigned long long packed) {
         out.top_ids[row * top + place] = packed_logit_index(packed);
         out.top_logprobs[row * top + place] = logprob_of(best_logit(packed), m, log2_sum);
     });
@@ -380,7 +430,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_join_kernel(
     float sum = 0.f, moment = 0.f;
     for (int p = tid; p < parts; p += LP_THREADS) {
         const float4 s = stats[p];
-        const float d = fmaxf((s.x - m) * LOG2E, -2000.f), w = __builtin_amdgcn_exp2f(d);
+        const float d = fmaxf(part_distance(s.x, m), -2000.f), w = __builtin_amdgcn_exp2f(d);
         sum = fmaf(w, s.y, sum);
         moment = fmaf(w, fmaf(d, s.y, s.z), moment);
     }
@@ -448,9 +498,9 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_join_kernel(
         if (done < parts) {
             for (int k = tid; k < top; k += LP_THREADS)
                 if (k >= have) so_far[k] = 0ull;
-            sorted_best(list, have, top, [&](int place, unsigned long long packed) { so_far[place] = packed; });
+            sorted_best<LP_THREADS>(list, have, top, [&](int place, unsigned long long packed) { so_far[place] = packed; });
         } else {
-            sorted_best(list, have, top, [&](int place, unsigned long long packed) {
+            sorted_best<LP_THREADS>(list, have, top, [&](int place, unsigned long long packed) {
                 out.top_ids[row * top + place] = packed_logit_index(packed);
                 out.top_logprobs[row * top + place] = logprob_of(best_logit(packed), m, log2_sum);
             });
@@ -459,21 +509,45 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_join_kernel(
 }
 
 // ---------------------------------------------------------------------------- how a call is cut
-// Parts of a row, and logits of a part.  A part holds at most `most` logits; with few rows it is smaller, down to 1,024.
-static void logprobs_cut(long long rows, int vocab, int dtype, bool aligned, int& parts, int& part_size, int& groups) {
-    const int n = dtype == CELEG_BF16 ? 8 : 4;
-    const int sizes[3] = {1, dtype == CELEG_BF16 ? 2 : 4, dtype == CELEG_BF16 ? 8 : 16};
-    for (int i = 0; i < 3; ++i) {
-        groups = sizes[i];
+// Parts of a row, logits of a part, and the threads of a workgroup with the groups that each holds.
+struct LogprobCut {
+    int parts, part_size, groups, threads;
+    LogprobCut(long long rows, int vocab, int dtype, bool aligned, int top) {
+        const bool bf = dtype == CELEG_BF16;
+        const int n = bf ? 8 : 4;
         // (rows that begin off a boundary need a group more)
-        const int most = LP_THREADS * groups * n - (aligned ? 0 : n);
-        parts = (vocab + most - 1) / most;
-        part_size = ((vocab + parts - 1) / parts + n - 1) / n * n;
-        if (part_size > most) part_size = most;
-        parts = (vocab + part_size - 1) / part_size;
-        if (rows * parts <= 1024 && parts <= 64) return;
+        const int lost = aligned ? 0 : n;
+        auto cut_into = [&](int most) {
+            parts = (vocab + most - 1) / most;
+            part_size = ((vocab + parts - 1) / parts + n - 1) / n * n;
+            if (part_size > most) part_size = most;
+            parts = (vocab + part_size - 1) / part_size;
+        };
+        // Up to 256 rows, one a compute unit: a row is a workgroup's, and nothing is joined.
+        if (rows <= 256) {
+            threads = LP_THREADS;
+            groups = bf ? 2 : 4;
+            cut_into(threads * groups * n - lost);
+            if (parts == 1) return;
+            threads = 1024;
+            // (where a row has fewer maxima than twice what is sought, the bound that they give is too low)
+            if (vocab >= 2 * top * n * 4)
+                for (int g : {bf ? 2 : 4, bf ? 4 : 8, bf ? 8 : 16}) {
+                    groups = g;
+                    cut_into(threads * groups * n - lost);
+                    // (long lists from few large parts are joined sooner than from many small ones)
+                    if (parts == 1 || (g * n == 64 && top > 32)) return;
+                }
+        }
+        // a part holds at most `most` logits; with few rows it is smaller, down to 1,024
+        threads = LP_THREADS;
+        for (int g : {1, bf ? 2 : 4, bf ? 8 : 16}) {
+            groups = g;
+            cut_into(threads * groups * n - lost);
+            if (rows * parts <= 1024 && parts <= 64) return;
+        }
     }
-}
+};
 
 static bool logprobs_aligned(const void* logits, int dtype, long long row_stride, long long rows) {
     const long long n = dtype == CELEG_BF16 ? 8 : 4;
@@ -484,10 +558,9 @@ static bool logprobs_aligned(const void* logits, int dtype, long long row_stride
 extern "C" size_t celeg_logprobs_workspace(int dtype, long long rows, int vocab, int per_row, int top) {
     size_t bytes = 0;
     for (int aligned = 0; aligned < 2; ++aligned) {
-        int parts, part_size, groups;
-        logprobs_cut(rows, vocab, dtype, aligned != 0, parts, part_size, groups);
-        const size_t all = static_cast<size_t>(rows) * parts;
-        const size_t b = parts > 1 ? all * 16 + all * top * 8 + all * per_row * 4 : 0;
+        const LogprobCut cut(rows, vocab, dtype, aligned != 0, top);
+        const size_t all = static_cast<size_t>(rows) * cut.parts;
+        const size_t b = cut.parts > 1 ? all * 16 + all * top * 8 + all * per_row * 4 : 0;
         bytes = b > bytes ? b : bytes;
     }
     return (bytes + 15) / 16 * 16;
@@ -496,12 +569,11 @@ extern "C" size_t celeg_logprobs_workspace(int dtype, long long rows, int vocab,
 extern "C" int celeg_logprobs_rows(const void* logits, int dtype, long long rows, int vocab, long long row_stride, const int* tokens,
                                    int per_row, int top, float* logprobs, int* ranks, float* entropy, int* top_ids,
                                    float* top_logprobs, void* workspace, hipStream_t stream) {
-    int parts, part_size, groups;
-    logprobs_cut(rows, vocab, dtype, logprobs_aligned(logits, dtype, row_stride, rows), parts, part_size, groups);
-    const size_t all = static_cast<size_t>(rows) * parts;
+    const LogprobCut cut(rows, vocab, dtype, logprobs_aligned(logits, dtype, row_stride, rows), top);
+    const size_t all = static_cast<size_t>(rows) * cut.parts;
     char* ws = static_cast<char*>(workspace);
     LogprobParts left{};
-    if (parts > 1) {
+    if (cut.parts > 1) {
         left.stats = reinterpret_cast<float4*>(ws);
         left.best = reinterpret_cast<unsigned long long*>(ws + all * 16);
         left.ranks = reinterpret_cast<int*>(ws + all * 16 + all * top * 8);
@@ -510,17 +582,26 @@ extern "C" int celeg_logprobs_rows(const void* logits, int dtype, long long rows
     auto run = [&](auto* x) {
         using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
         constexpr bool B = std::is_same<T, bf16>::value;
-        const dim3 grid(static_cast<unsigned>(all)), block(LP_THREADS);
-        auto part = [&](auto count) {
-            logprobs_part_kernel<T, decltype(count)::value><<<grid, block, 0, stream>>>(x, row_stride, tokens, vocab, per_row, top, parts,
-                                                                                      part_size, left, out);
+        auto part = [&](auto groups, auto threads) {
+            constexpr int THREADS = decltype(threads)::value;
+            logprobs_part_kernel<T, decltype(groups)::value, THREADS><<<dim3(static_cast<unsigned>(all)), dim3(THREADS), 0, stream>>>(
+                x, row_stride, tokens, vocab, per_row, top, cut.parts, cut.part_size, left, out);
         };
-        if (groups == 1) part(std::integral_constant<int, 1>{});
-        else if (groups == (B ? 2 : 4)) part(std::integral_constant<int, B ? 2 : 4>{});
-        else part(std::integral_constant<int, B ? 8 : 16>{});
-        if (parts > 1)
-            logprobs_join_kernel<T><<<dim3(static_cast<unsigned>(rows)), block, 0, stream>>>(x, row_stride, tokens, vocab, per_row, top, parts,
-                                                                                           left, out);
+        auto of = [](auto value) { return value; };
+        if (cut.threads == 1024) {
+            const auto threads = of(std::integral_constant<int, 1024>{});
+            if (cut.groups == (B ? 2 : 4)) part(std::integral_constant<int, B ? 2 : 4>{}, threads);
+            else if (cut.groups == (B ? 4 : 8)) part(std::integral_constant<int, B ? 4 : 8>{}, threads);
+            else part(std::integral_constant<int, B ? 8 : 16>{}, threads);
+        } else {
+            const auto threads = of(std::integral_constant<int, LP_THREADS>{});
+            if (cut.groups == 1) part(std::integral_constant<int, 1>{}, threads);
+            else if (cut.groups == (B ? 2 : 4)) part(std::integral_constant<int, B ? 2 : 4>{}, threads);
+            else part(std::integral_constant<int, B ? 8 : 16>{}, threads);
+        }
+        if (cut.parts > 1)
+            logprobs_join_kernel<T><<<dim3(static_cast<unsigned>(rows)), dim3(LP_THREADS), 0, stream>>>(x, row_stride, tokens, vocab, per_row, top,
+                                                                                                        cut.parts, left, out);
     };
     if (dtype == CELEG_BF16) run(static_cast<const bf16*>(logits));
     else run(static_cast<const float*>(logits));
