@@ -834,15 +834,22 @@ extern "C" int celeg_tree_attention_fast_ok(int head_dim, int page_tokens) {
     return (head_dim == 32 || head_dim == 64 || head_dim == 96 || head_dim == 128) && page_tokens >= 16 && (page_tokens & (page_tokens - 1)) == 0;
 }
 
-// Parts that the contexts are cut into: as many workgroups as the chip holds at a time, each wavefront (each workgroup that stages:
-// two) with a round at least.  More of them cost more to join than an even end gains (as above, 512 workgroups of 128 rows: 446 us, 640:
-// 470, 1,024: 485).
+// Parts that the contexts are cut into.
+//   Few rounds are one workgroup's: up to 12 (4 where keys are staged) a second kernel costs more than the wait (1 request of 8 nodes,
+// 16 heads of 64 on 8, behind 700: 9.2 us, in 3 parts 9.8, and a launch less for the host; behind 1,500: 13.3 and 10.6).
+//   More: 256 workgroups, one a compute unit, each wavefront (each workgroup that stages: two) with a round at least: a second one beside it
+// gains less than its part costs to join (4 trees of 8 behind 6,000, 32 heads of 64 on 8: 20.0 us, of 512 workgroups 22.9; heads
+// of 128 29.7 and 34.9; 4 of 26 behind 2,500, staged: 16.7 and 21.3).  Staged rounds in long parts, more than 16 of them, gain more (8
+// of 26 behind 16,000: 64 us, of 256 workgroups 80; behind 2,500 25 and 25).
 extern "C" int celeg_tree_attention_parts(int dtype, int head_dim, int requests, int kv_heads, int group, int max_nodes, int max_context) {
     const int rows = max_nodes * group;
     const TreeForm form = tree_form(dtype, head_dim, rows);
     const long long groups = static_cast<long long>(requests) * kv_heads * ((rows + form.rows - 1) / form.rows);
     const long long rounds = (static_cast<long long>(max_context) + max_nodes + form.keys - 1) / form.keys;
-    return static_cast<int>(std::max(1LL, std::min({(256 * form.resident + groups - 1) / groups, form.staged ? (rounds + 1) / 2 : (rounds + 3) / 4, 64LL})));
+    if (rounds <= (form.staged ? 4 : 12)) return 1;
+    long long parts = (256 + groups - 1) / groups;
+    if (form.staged && form.resident > 1 && rounds > 16 * parts) parts = (256 * form.resident + groups - 1) / groups;
+    return static_cast<int>(std::max(1LL, std::min({parts, form.staged ? (rounds + 1) / 2 : (rounds + 3) / 4, 64LL})));
 }
 
 extern "C" int celeg_tree_attention_fast(const void* q, int ldq, int dtype, const void* k_pool, const void* v_pool, int n_pages, int n_layers,
