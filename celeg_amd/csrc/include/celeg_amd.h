@@ -295,7 +295,8 @@ celeg_status celeg_token_logprobs(const celeg_token_logprobs_args* args, void* w
  * root).  A node sees the context, its ancestors and itself, with a window only what stands fewer than `window` positions
  * before its own, starts[r] + depth.  out = softmax(scale q . k) v [rows, heads * head_dim], in the pages' dtype like q (rows
  * q_stride elements apart).  Rows of no request, of a request behind max_nodes, or of a slot outside the table are left as
- * they were.  What a node does not see may hold anything, infinities and NaN included. */
+ * they were.  What a node does not see may hold anything, infinities and NaN included; a node that sees nothing (none of its
+ * places has a page) gets zeros. */
 typedef struct celeg_tree_attention_args {
     size_t struct_size;
     const void* q;

@@ -2,7 +2,7 @@
 //
 // A request's context lies at the places 0 .. start - 1 of its pages, the keys and values of its tree's nodes behind it, node i
 // at place start + i.  Node i stands at position start + depth(i); it sees the context, its ancestors and itself, of them (with a
-// window w) the keys at positions above its own less w.  out = softmax(scale q . k) v over what it sees.
+// window w) the keys at positions above its own less w.  out = softmax(scale q . k) v over what it sees, zeros if that is nothing.
 // parents[row]: the index inside its request's tree of a node's parent; what is not an index below the node's own makes it a root.
 //   K [pages, layers, kv_heads, page_tokens, head_dim], V [pages, layers, kv_heads, head_dim, page_tokens]
 //
@@ -346,7 +346,7 @@ template <typename T, int HD>
 __device__ __forceinline__ void tree_store(const TreeArgs& a, size_t row, int head, int part, int qd, float m, float l, const tree_f4 (&o)[HD / 16]) {
     if (a.parts == 1) {
         T* to = static_cast<T*>(a.out) + (row * a.heads + head) * HD + 4 * qd;
-        const float inverse = 1.f / l;
+        const float inverse = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
         for (int dt = 0; dt < HD / 16; ++dt) {
             const float x[4] = {o[dt][0] * inverse, o[dt][1] * inverse, o[dt][2] * inverse, o[dt][3] * inverse};
@@ -806,7 +806,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeArgs a) {
     T* to = static_cast<T*>(a.out) + (static_cast<size_t>(first + node) * a.heads + head) * HD;
 #pragma unroll
     for (int e = 0; e < PER; ++e)
-        if (lane + 64 * e < HD) to[lane + 64 * e] = from_float<T>(o[e] / sum);
+        if (lane + 64 * e < HD) to[lane + 64 * e] = from_float<T>(sum == 0.f ? 0.f : o[e] / sum);
 }
 
 // The form of a launch: whether keys are staged, row tiles of a wavefront, rows of a workgroup, keys of a round, and workgroups
@@ -994,7 +994,7 @@ __global__ __launch_bounds__(64) void tree_attention_general_kernel(
     T* orow = out + static_cast<size_t>(first + node) * heads * head_dim + static_cast<size_t>(h) * head_dim;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        if (lane + 64 * e < head_dim) orow[lane + 64 * e] = from_float<T>(o[e] / l);
+        if (lane + 64 * e < head_dim) orow[lane + 64 * e] = from_float<T>(l == 0.f ? 0.f : o[e] / l);
 }
 
 extern "C" int celeg_tree_attention_general(const void* q, int ldq, int dtype, const void* k_pool, const void* v_pool, int n_pages,

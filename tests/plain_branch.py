@@ -67,7 +67,7 @@ def tree_attention(q, k, v, table, layer, slots, starts, offsets, parents, scale
             low = max(0, starts[r] + depth - window + 1) if window else 0
             places = list(range(low, starts[r])) + sorted(starts[r] + a for up, a in enumerate(ways[i]) if not window or up < window)
             places = [p for p in places if p // page < len(pages) and 0 <= pages[p // page] < k.shape[0]]
-            where, at = torch.tensor([pages[p // page] for p in places]), torch.tensor([p % page for p in places])
+            where, at = (torch.tensor(x, dtype=torch.long) for x in ([pages[p // page] for p in places], [p % page for p in places]))
             for h in range(heads):
                 kh = k[where, layer, h // (heads // kv_heads), at].to(F64)
                 vh = v[where, layer, h // (heads // kv_heads), :, at].to(F64)

@@ -285,6 +285,20 @@ def test_tree_slots_and_pages_outside(dtype):
     t.check()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("page", [16, 12])
+@pytest.mark.parametrize("context,nodes", [(20, 3), (2000, 5), (300, 60)])
+def test_tree_rows_that_see_nothing(context, nodes, page, dtype):
+    t = Trees((context, 40), (nodes, 4), 8, 2, 64, dtype, layers=1, page=page, seed=17)
+    t.table[0] = -1                                     # (the request has rows, and no page)
+    got = t.check(max_context=context)
+    assert (got[:nodes] == 0).all() and (got[nodes:nodes + 4] != 0).any()
+    t = Trees((context,), (nodes,), 8, 2, 64, dtype, layers=1, page=page, seed=18, width=-(-(context + nodes) // page))
+    t.starts[0] = t.table.shape[1] * page + 7           # all of the tree, and with the window what it sees, behind the table
+    got = t.check(window=5)
+    assert (got[:nodes] == 0).all()
+
+
 def test_tree_rows_of_a_request_behind_max_nodes():
     t = Trees((30, 20), (9, 3), 4, 2, 64, BF16, seed=15)
     t.check(max_nodes=5)
