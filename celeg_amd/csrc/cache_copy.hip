@@ -68,7 +68,8 @@ struct MoveRequest {
         from_slot = a.src_slots[r];
         to_slot = a.dst_slots[r];
         first = max(a.offsets[r], 0);
-        count = min(a.offsets[r + 1], a.n_places) - first;
+        const int to = min(a.offsets[r + 1], a.n_places);
+        count = to > first ? to - first : 0;
         start = a.dst_starts[r];
         ok = from_slot >= 0 && from_slot < a.table_rows && to_slot >= 0 && to_slot < a.table_rows && start >= 0 && count > 0;
     }

@@ -2,6 +2,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 
 #include "kernels.hpp"
 
@@ -11,12 +12,18 @@ namespace {
 void need(bool ok, const char* message) {
     if (!ok) throw ArgumentError(message);
 }
+// addresses of values of `size` bytes each
+void aligned(std::initializer_list<const void*> addresses, size_t size, const char* message) {
+    for (const void* p : addresses) need(reinterpret_cast<uintptr_t>(p) % size == 0, message);
+}
 void floats(DType dtype, const char* message) { need(dtype == DType::F32 || dtype == DType::BF16, message); }
 
 // the pages and the table of a group, as the kernels address them
 void check_cache(const KVView& kv) {
     floats(kv.dtype, "cache: the pages are float32 or bfloat16");
     need(kv.k && kv.table, "cache: the pages or the table are missing");
+    aligned({kv.k, kv.v}, dtype_size(kv.dtype), "cache: the pages must lie on a boundary of their type");
+    aligned({kv.table}, 4, "cache: the table must lie on a boundary of 4 bytes");
     need(kv.n_pages > 0 && kv.n_layers > 0 && kv.kv_heads > 0 && kv.page_tokens > 0 && kv.head_dim > 0 && kv.v_head_dim >= 0 &&
              kv.table_rows > 0 && kv.table_stride > 0, "cache: sizes must be positive");
     need((kv.v_head_dim > 0) == (kv.v != nullptr), "cache: values and their width come together (keys only: neither)");
@@ -48,6 +55,8 @@ static void check(const TokenLogprobs& a) {
     need(a.logits != nullptr, "token_logprobs: the logits are missing");
     need(a.per_row == 0 || (a.tokens && a.logprobs && a.ranks), "token_logprobs: tokens, logprobs and ranks come together");
     need(a.top == 0 || (a.top_ids && a.top_logprobs), "token_logprobs: top_ids and top_logprobs are missing");
+    aligned({a.logits}, dtype_size(a.dtype), "token_logprobs: logits must lie on a boundary of their type");
+    aligned({a.tokens, a.logprobs, a.ranks, a.entropy, a.top_ids, a.top_logprobs}, 4, "token_logprobs: lists and results must lie on boundaries of 4 bytes");
 }
 
 size_t token_logprobs_workspace(const TokenLogprobs& a) {
@@ -85,6 +94,8 @@ static void check(const TreeAttention& a, const KVView& kv) {
     check_sizes(a, kv);
     if (a.rows == 0 || a.requests == 0) return;
     need(a.q && a.out && a.slots && a.starts && a.offsets && a.parents, "tree_attention: an argument is missing");
+    aligned({a.q, a.out}, dtype_size(kv.dtype), "tree_attention: q and out must lie on a boundary of their type");
+    aligned({a.slots, a.starts, a.offsets, a.parents}, 4, "tree_attention: lists must lie on boundaries of 4 bytes");
 }
 
 // Parts that the contexts are cut into, 0: the kernel for any sizes, which reads single values.
@@ -130,6 +141,7 @@ void move_tokens(const MoveTokens& a, const KVView& kv, hipStream_t stream) {
     need(a.requests >= 0 && a.n_places >= 0, "move_tokens: negative counts");
     if (a.requests == 0 || a.n_places == 0) return;
     need(a.src_slots && a.dst_slots && a.offsets && a.places && a.dst_starts, "move_tokens: an argument is missing");
+    aligned({a.src_slots, a.dst_slots, a.offsets, a.places, a.dst_starts}, 4, "move_tokens: lists must lie on boundaries of 4 bytes");
     kernel_check(celeg_move_token_list(kv.k, kv.v, static_cast<int>(kv.dtype), kv.n_pages, kv.n_layers, kv.kv_heads, kv.page_tokens,
                                        kv.head_dim, kv.v_head_dim, kv.table, kv.table_rows, kv.table_stride, a.src_slots, a.dst_slots,
                                        a.offsets, a.places, a.dst_starts, a.requests, a.n_places, stream), "move_tokens");
@@ -140,6 +152,7 @@ void copy_pages(const KVView& kv, const int* src, const int* dst, int n, hipStre
     need(n >= 0, "copy_pages: a negative count");
     if (n == 0) return;
     need(src && dst, "copy_pages: the lists of pages are missing");
+    aligned({src, dst}, 4, "copy_pages: lists must lie on boundaries of 4 bytes");
     const size_t per_dim = static_cast<size_t>(kv.n_layers) * kv.kv_heads * kv.page_tokens * dtype_size(kv.dtype);
     kernel_check(celeg_copy_page_list(kv.k, kv.v, per_dim * kv.head_dim, per_dim * kv.v_head_dim, kv.n_pages, src, dst, n, stream),
                  "copy_pages");

@@ -11,6 +11,7 @@
 // sum and output of its own, and meet in LDS; long contexts are cut into parts for as many workgroups, which a second kernel joins.
 #include "common.h"
 #include <algorithm>
+#include <climits>
 
 #define TREE_MAX_NODES 256
 
@@ -27,6 +28,15 @@ __device__ __forceinline__ int tree_depth(const int* parents, int node) {
         ++depth;
     }
 }
+
+// Rows of request r from `first` on that the arrays hold (lists may name anything).
+__device__ __forceinline__ int tree_count(const int* offsets, int r, int n_rows, int max_nodes) {
+    const int first = offsets[r], to = min(offsets[r + 1], n_rows);
+    return first >= 0 && to > first ? min(to - first, max_nodes) : 0;
+}
+
+// The context's tokens, so far below the largest number that nothing added to it passes that.
+__device__ __forceinline__ int tree_start(const int* starts, int r) { return min(max(starts[r], 0), INT_MAX - 4096); }
 
 // ---------------------------------------------------------------------------- on the matrix cores
 struct TreeArgs {
@@ -167,14 +177,14 @@ struct TreeRequest {
     __device__ __forceinline__ TreeRequest(const TreeArgs& a, int r) {
         // (the same for all lanes: said so that they take no vector registers)
         first = __builtin_amdgcn_readfirstlane(a.offsets[r]);
-        count = __builtin_amdgcn_readfirstlane(min(min(a.offsets[r + 1], a.n_rows) - first, a.max_nodes));
+        count = __builtin_amdgcn_readfirstlane(tree_count(a.offsets, r, a.n_rows, a.max_nodes));
         slot = __builtin_amdgcn_readfirstlane(a.slots[r]);
-        start = __builtin_amdgcn_readfirstlane(max(a.starts[r], 0));
+        start = __builtin_amdgcn_readfirstlane(tree_start(a.starts, r));
         rows = count * a.group;
         // (places behind what the table holds are seen by nobody)
         const int room = a.table_stride << a.page_shift;
         end = start < room ? min(start + count, room) : room;
-        ok = first >= 0 && count > 0 && slot >= 0 && slot < a.table_rows;
+        ok = count > 0 && slot >= 0 && slot < a.table_rows;
         pages = a.table + static_cast<size_t>(ok ? slot : 0) * a.table_stride;
     }
 };
@@ -787,8 +797,8 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeArgs a) {
     const int head = static_cast<int>(id % a.heads), node = static_cast<int>(id / a.heads % a.max_nodes);
     const long long r = id / (static_cast<long long>(a.heads) * a.max_nodes);
     if (r >= a.requests) return;
-    const int first = a.offsets[r], count = min(a.offsets[r + 1], a.n_rows) - first, slot = a.slots[r];
-    if (first < 0 || node >= count || slot < 0 || slot >= a.table_rows) return;
+    const int first = a.offsets[r], slot = a.slots[r];
+    if (node >= tree_count(a.offsets, r, a.n_rows, a.max_nodes) || slot < 0 || slot >= a.table_rows) return;
     const size_t at = (static_cast<size_t>(first + node) * a.heads + head) * a.parts;
     float high = -INFINITY;
     for (int p = lane; p < a.parts; p += 64) high = fmaxf(high, a.ws_ml[2 * (at + p)]);
@@ -931,9 +941,9 @@ __global__ __launch_bounds__(64) void tree_attention_general_kernel(
     const int* __restrict__ slots, const int* __restrict__ starts, const int* __restrict__ offsets, const int* __restrict__ parents,
     int n_rows, int max_nodes, float scale, int window, T* __restrict__ out) {
     const int r = blockIdx.y / max_nodes, node = blockIdx.y % max_nodes, h = blockIdx.x, lane = threadIdx.x;
-    const int first = offsets[r], count = min(offsets[r + 1] - first, max_nodes);
-    const int slot = slots[r], start = max(starts[r], 0);
-    if (node >= count || first < 0 || first + node >= n_rows || slot < 0 || slot >= table_rows) return;
+    const int first = offsets[r], count = tree_count(offsets, r, n_rows, max_nodes);
+    const int slot = slots[r], start = tree_start(starts, r);
+    if (node >= count || slot < 0 || slot >= table_rows) return;
     const int* up = parents + first;
     const int depth = tree_depth(up, node), low = window > 0 ? max(0, start + depth - window + 1) : 0;
     __shared__ float qs[256];
@@ -952,7 +962,8 @@ __global__ __launch_bounds__(64) void tree_attention_general_kernel(
         }
     }
     __syncthreads();
-    const int end = start + count;
+    const int room = table_stride * page_tokens;       // (below 2^31: checked by the host; places behind it are seen by nobody)
+    const int end = start < room ? min(start + count, room) : room;
     const size_t per_head = static_cast<size_t>(page_tokens) * head_dim;
     const size_t head_block = (static_cast<size_t>(layer) * kv_heads + h / (heads / kv_heads)) * per_head;
     const size_t page_size = static_cast<size_t>(n_layers) * kv_heads * per_head;

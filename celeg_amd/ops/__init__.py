@@ -79,6 +79,13 @@ class PagedCache:
             table.shape[0], table.shape[1])
         self._ref = ctypes.byref(self._struct)
 
+    def _here(self):
+        """What the library is given, as long as the tensors are where they were."""
+        s = self._struct
+        if self.k.data_ptr() != s.k or (self.v is not None and self.v.data_ptr() != s.v) or self.table.data_ptr() != s.table:
+            _refuse("the cache's tensors have moved: make a PagedCache of them anew")
+        return self._ref
+
 
 class TokenLogprobs(NamedTuple):
     logprobs: Optional[torch.Tensor]         # float32 [rows, n], shaped as the tokens were given (None: no tokens)
@@ -155,9 +162,10 @@ def tree_attention(q: torch.Tensor, cache: PagedCache, layer: int, slots: torch.
         _ints(parents, "parents", rows, device), cache.head_dim ** -0.5 if scale is None else scale, window,
         min(max(rows, 1), MAX_TREE_NODES) if max_nodes is None else max_nodes, max_context)
     lib, ref, size = native.lib(), ctypes.byref(args), ctypes.c_size_t()
-    native.check(lib.celeg_tree_attention_workspace(ref, cache._ref, ctypes.byref(size)))
+    pages = cache._here()
+    native.check(lib.celeg_tree_attention_workspace(ref, pages, ctypes.byref(size)))
     workspace = torch.empty(size.value, dtype=torch.uint8, device=device) if size.value else None
-    _call(device, lib.celeg_tree_attention, ref, cache._ref, workspace.data_ptr() if size.value else None, size.value)
+    _call(device, lib.celeg_tree_attention, ref, pages, workspace.data_ptr() if size.value else None, size.value)
     return out
 
 
@@ -174,7 +182,7 @@ def move_tokens(cache: PagedCache, src_slots: torch.Tensor, dst_slots: torch.Ten
     if not isinstance(places, torch.Tensor) or places.dim() != 1:
         _refuse("places must be int32 [entries]")
     requests = src_slots.shape[0]
-    _call(device, native.lib().celeg_move_tokens, cache._ref, requests, _ints(src_slots, "src_slots", requests, device),
+    _call(device, native.lib().celeg_move_tokens, cache._here(), requests, _ints(src_slots, "src_slots", requests, device),
           _ints(dst_slots, "dst_slots", requests, device), _ints(offsets, "offsets", requests + 1, device),
           _ints(places, "places", None, device), places.shape[0], _ints(dst_starts, "dst_starts", requests, device))
 
@@ -186,7 +194,7 @@ def copy_pages(cache: PagedCache, src: torch.Tensor, dst: torch.Tensor) -> None:
     if not isinstance(src, torch.Tensor) or src.dim() != 1:
         _refuse("src must be int32 [pairs]")
     n = src.shape[0]
-    _call(cache.device, native.lib().celeg_copy_pages, cache._ref, _ints(src, "src", n, cache.device), _ints(dst, "dst", n, cache.device), n)
+    _call(cache.device, native.lib().celeg_copy_pages, cache._here(), _ints(src, "src", n, cache.device), _ints(dst, "dst", n, cache.device), n)
 
 
 __all__ = ["PagedCache", "TokenLogprobs", "token_logprobs", "tree_attention", "move_tokens", "copy_pages", "MAX_TOKENS_PER_ROW",

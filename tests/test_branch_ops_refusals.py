@@ -110,6 +110,21 @@ def test_lists():
     refused(lib.celeg_copy_pages, ctypes.byref(c), ADDRESS, None, 1, None)
 
 
+def test_addresses_off_their_types():
+    lib, odd = native.lib(), ADDRESS + 1
+    for name in ("logits", "tokens", "logprobs", "ranks", "entropy", "top_ids", "top_logprobs"):
+        assert "boundar" in refused(lib.celeg_token_logprobs, ctypes.byref(logprobs(**{name: odd})), ADDRESS, 1 << 40, None)
+    for name in ("q", "out", "slots", "starts", "offsets", "parents"):
+        assert "boundar" in refused(lib.celeg_tree_attention, ctypes.byref(tree(**{name: odd})), ctypes.byref(cache()), ADDRESS, 1 << 40, None)
+    for name in ("k", "v", "table"):
+        assert "boundar" in refused(lib.celeg_copy_pages, ctypes.byref(cache(**{name: odd})), ADDRESS, ADDRESS, 1, None)
+    for at in range(5):
+        lists = [ADDRESS] * 5
+        lists[at] = odd
+        assert "boundar" in refused(lib.celeg_move_tokens, ctypes.byref(cache()), 1, lists[0], lists[1], lists[2], lists[3], 1, lists[4], None)
+    assert "boundar" in refused(lib.celeg_copy_pages, ctypes.byref(cache()), ADDRESS, odd, 1, None)
+
+
 def test_nothing_to_do():
     lib = native.lib()
     native.check(lib.celeg_token_logprobs(ctypes.byref(logprobs(rows=0, logits=None, tokens=None)), None, 0, None))

@@ -299,6 +299,26 @@ def test_tree_rows_that_see_nothing(context, nodes, page, dtype):
     assert (got[:nodes] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("page,nodes", [(16, 4), (16, 40), (12, 4)])
+def test_tree_lists_that_name_anything(page, nodes, dtype):
+    """Offsets that end before they begin or behind the rows, starts at both ends of the numbers: nothing but the request's own rows
+    is written."""
+    for bad in (-2 ** 31, -1, 2 ** 31 - 1):
+        t = Trees((30, 40), (nodes, 5), 8, 2, 64, dtype, page=page, seed=19)
+        t.offsets[1] = bad                              # the first request's end, the second's beginning
+        got = t.run(max_nodes=nodes).cpu()
+        assert (got[t.offsets[2]:] == 7.0).all() if bad < 0 else got.isfinite().all()
+        t = Trees((30, 40), (nodes, 5), 8, 2, 64, dtype, page=page, seed=19)
+        want = t.run(max_nodes=nodes).cpu()
+        t.starts[0] = bad
+        for window in (0, 9):
+            got = t.run(max_nodes=nodes, window=window).cpu()
+            assert (got[t.rows:] == 7.0).all()
+            if not window:
+                assert torch.equal(got[nodes:nodes + 5], want[nodes:nodes + 5])
+
+
 def test_tree_rows_of_a_request_behind_max_nodes():
     t = Trees((30, 20), (9, 3), 4, 2, 64, BF16, seed=15)
     t.check(max_nodes=5)
@@ -378,6 +398,29 @@ def test_move_tokens_leaves_out_what_is_not_there():
     check_move(k, v, table, [2], [0], [0, 40], list(range(40)), [20])
     check_move(k, v, table, [0], [1], [0, 6], [-1, 95, 96, 2 ** 31 - 1, -2 ** 31, 3], [85])
     check_move(k, v, table, [0], [1], [0, 4], [1, 2, 3, 4], [94])
+
+
+def test_move_tokens_lists_that_name_anything():
+    k, v, table = cache_of(20, 2, 2, 16, 64, 64, BF16, 5, 3, 6)
+    for bad in (-2 ** 31, -1, 2 ** 31 - 1):
+        gk, gv = k.cuda(), v.cuda()
+        ints = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+        cache = ops.PagedCache(gk, gv, table.cuda())
+        ops.move_tokens(cache, ints([0, 1]), ints([2, 2]), ints([3, bad, 3]), ints([1, 2, 3, 4]), ints([0, 40]))
+        if bad < 0:                                     # (the first request has nothing; the second's entries begin at 0)
+            want = moved(k, v, table, [1], [2], [0, 3], [1, 2, 3], [40])
+        else:                                           # (the first one's entries end with the list)
+            want = moved(k, v, table, [0], [2], [0, 1], [4], [0])
+        assert torch.equal(gk.cpu(), want[0]) and torch.equal(gv.cpu(), want[1])
+
+
+def test_a_cache_whose_tensors_moved():
+    k, v, table = (x.cuda() for x in cache_of(4, 1, 1, 16, 32, 32, BF16, 6, 1, 4))
+    cache, one = ops.PagedCache(k, v, table), torch.zeros(1, dtype=torch.int32, device="cuda")
+    ops.copy_pages(cache, one, one)
+    cache.v = v.clone()
+    with pytest.raises(ValueError, match="moved"):
+        ops.copy_pages(cache, one, one)
 
 
 def test_move_tokens_many_in_place():
