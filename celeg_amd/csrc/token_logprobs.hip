@@ -83,7 +83,9 @@ __device__ __forceinline__ float logprob_of(float x, float m, float log2_sum) {
     return d == -INFINITY ? (x - m) - log2_sum * LN2 : (d - log2_sum) * LN2;       // (what is far below may fit in nats alone)
 }
 
-// Of n packed logits in `list` (all different), the `top` largest in falling order: put(place, packed).  All threads call it.
+// Of n packed logits in `list` (all different), the `top` largest in falling order: put(place, packed).  All threads call it, behind a
+// barrier; there is one more in it.  They are counted against one another eight at a time, whose reads are under way together (the list
+// has room for eight more, which are made 0): one at a time 128 best took twice as long as all the rest.
 // The same of a part's largest, as the part has it: its sums are against the rounded product.
 __device__ __forceinline__ float part_distance(float part, float m) {
     if (!(fabsf(part) < LP_FITS && fabsf(m) < LP_FITS)) return (part - m) * LOG2E;
@@ -93,11 +95,20 @@ __device__ __forceinline__ float part_distance(float part, float m) {
 }
 
 template <int THREADS, typename F>
-__device__ __forceinline__ void sorted_best(const unsigned long long* list, int n, int top, F put) {
+__device__ __forceinline__ void sorted_best(unsigned long long* list, int n, int top, F put) {
+    typedef unsigned long long two __attribute__((ext_vector_type(2)));
+    if (threadIdx.x < 8) list[n + threadIdx.x] = 0ull;
+    __syncthreads();
     for (int i = threadIdx.x; i < n; i += THREADS) {
         const unsigned long long mine = list[i];
         int ahead = 0;
-        for (int j = 0; j < n; ++j) ahead += list[j] > mine;
+        for (int j = 0; j < n; j += 8) {
+            two of[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) of[e] = *reinterpret_cast<const two*>(list + j + 2 * e);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) ahead += (of[e][0] > mine) + (of[e][1] > mine);
+        }
         if (ahead < top) put(ahead, mine);
     }
 }
@@ -171,7 +182,7 @@ __global__ __launch_bounds__(THREADS, 1024 / THREADS) void logprobs_part_kernel(
     __shared__ int n_groups, count, counts[2 * WAVES];
     __shared__ Group hit[LP_GROUPS];
     __shared__ int hit_at[LP_GROUPS];
-    __shared__ unsigned long long list[LP_LIST];
+    __shared__ __align__(16) unsigned long long list[LP_LIST + 8];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int part = blockIdx.x % parts;
     const size_t row = blockIdx.x / parts;
@@ -263,10 +274,14 @@ __global__ __launch_bounds__(THREADS, 1024 / THREADS) void logprobs_part_kernel(
         const int n = few ? 64 : 256;
         const float mine = maxima[tid];
         int above = 0;
-        for (int j = 0; j < n; j += 4) {
-            const lp_f4 o = *reinterpret_cast<const lp_f4*>(maxima + j);
+        for (int j = 0; j < n; j += 32) {
+            lp_f4 o[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) above += o[e] > mine;
+            for (int x = 0; x < 8; ++x) o[x] = *reinterpret_cast<const lp_f4*>(maxima + j + 4 * x);
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) above += o[x][e] > mine;
         }
         const float least = -wave_max(above < top ? -mine : -INFINITY);
         if (lane == 0) bounds[wave] = least;
@@ -404,7 +419,7 @@ template <typename T>
 __global__ __launch_bounds__(LP_THREADS) void logprobs_join_kernel(
     const T* __restrict__ logits, long long row_stride, const int* __restrict__ tokens, int vocab, int per_row, int top, int parts,
     const LogprobParts left, const LogprobOut out) {
-    __shared__ unsigned long long all[LP_JOIN], list[LP_JOIN], so_far[LP_MAX_TOP];
+    __shared__ __align__(16) unsigned long long all[LP_JOIN], list[LP_JOIN + 8], so_far[LP_MAX_TOP];
     __shared__ unsigned long long bound_shared;
     __shared__ float wave_of[3][LP_WAVES];
     __shared__ int count;
@@ -482,9 +497,12 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_join_kernel(
         for (int i = tid; i < lists; i += LP_THREADS) {
             const unsigned long long mine = all[i * top + depth - 1];
             int ahead = 0;
-            for (int j = 0; j < lists; ++j) {
-                const unsigned long long other = all[j * top + depth - 1];
-                ahead += other > mine || (other == mine && j < i);
+            for (int j = 0; j < lists; j += 8) {
+                unsigned long long other[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) other[e] = all[min(j + e, lists - 1) * top + depth - 1];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) ahead += j + e < lists && (other[e] > mine || (other[e] == mine && j + e < i));
             }
             if (ahead == nth - 1 && mine > 0ull) bound_shared = mine;       // (0: a list has no such entry; then everything counts)
         }
