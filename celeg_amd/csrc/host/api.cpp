@@ -512,6 +512,7 @@ celeg_status celeg_model_step_logprobs(celeg_model* model, int32_t n_entries, co
         a.entropy = out + 2 * given;
         a.top_ids = reinterpret_cast<int*>(out + 2 * given + n);
         a.top_logprobs = out + 2 * given + n + best;
+        lm.rt->ops.took(Path::TokenLogprobs);
         token_logprobs(a, block.as<char>() + at_workspace, workspace, lm.stream);
         std::vector<float> host(back);
         CELEG_HIP(hipMemcpyAsync(host.data(), out, back * 4, hipMemcpyDeviceToHost, lm.stream));

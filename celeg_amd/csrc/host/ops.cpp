@@ -80,6 +80,8 @@ const char* path_name(Path p) {
         case Path::FusedRows: return "fused_rows";
         case Path::FusedStaged: return "fused_staged";
         case Path::ArgmaxMerged: return "argmax_merged";
+        case Path::AttentionTrees: return "attention_trees";
+        case Path::TokenLogprobs: return "token_logprobs";
         case Path::Tiled: return "tiled";
         case Path::TiledQkv: return "tiled_qkv";
         default: return "?";

@@ -114,7 +114,7 @@ struct StepPrologue {
 // path it was meant to take.
 enum class Path : int {
     AttentionDecode = 0, AttentionDecodeFresh, AttentionRows, AttentionGeneral, AttentionSigmoid, AttentionSigmoidRows, AttentionSigmoidDecode, DeltaRule, AttentionLatent, AttentionLatentRows, AttentionLatentDecode, AttentionBiased, AttentionBiasedRows, AttentionBiasedDecode, ChannelScan, MatrixMemory, MatrixMemoryRows, MatrixMemoryStep, DecayScan, DecayScanRows, DecayScanStep, LinearRecurrentUnit, RoutedExperts, LinearF32, LinearF32Fused, LinearLibrary, LinearFewRows, LinearStandIn,
-    FusedSliced, FusedRows, FusedStaged, Tiled, TiledQkv, ArgmaxMerged, Count
+    FusedSliced, FusedRows, FusedStaged, Tiled, TiledQkv, ArgmaxMerged, AttentionTrees, TokenLogprobs, Count
 };
 const char* path_name(Path p);
 

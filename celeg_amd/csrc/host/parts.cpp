@@ -515,6 +515,7 @@ private:
             const size_t needed = tree_attention_workspace(a, *cache.kv);
             size_t bytes = needed ? size_t(1) << 16 : 0;
             while (bytes < needed) bytes *= 2;
+            rt.ops.took(Path::AttentionTrees);
             tree_attention(a, *cache.kv, bytes ? rt.ws.raw("tree_parts", bytes) : nullptr, bytes, rt.stream);
             return attended;
         }

@@ -73,6 +73,7 @@ def test_every_path_of_a_tree_is_as_if_it_were_alone(attention_folders, name, dt
         assert lm.cache.prepare(slot, len(context), len(tokens))
         entries.append(StepEntry(slot, len(context), tokens, range(len(tokens)), parents))
     got = lm.runner.step(entries)
+    assert lm.paths()["attention_trees"] == cfg["num_hidden_layers"]
     row = 0
     for context, (parents, tokens) in zip(contexts, trees):
         parents = parents or [i - 1 for i in range(len(tokens))]
@@ -173,6 +174,7 @@ def test_a_sequence_is_scored(model_folders, name, dtype, stored):
     logits = plain.model_logits(cfg, W, tokens)[:-1].double()
     want = torch.log_softmax(logits, 1)
     got = lm.score(tokens, top=5, portion=23)
+    assert lm.paths()["token_logprobs"] == 5
     at = torch.tensor(tokens[1:])
     # (a log probability is off by as much as two logits are)
     assert_close(got.logprobs[:, 0], want.gather(1, at[:, None])[:, 0], dtype)
