@@ -800,18 +800,36 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeArgs a) {
     const int first = a.offsets[r], slot = a.slots[r];
     if (node >= tree_count(a.offsets, r, a.n_rows, a.max_nodes) || slot < 0 || slot >= a.table_rows) return;
     const size_t at = (static_cast<size_t>(first + node) * a.heads + head) * a.parts;
-    float high = -INFINITY;
-    for (int p = lane; p < a.parts; p += 64) high = fmaxf(high, a.ws_ml[2 * (at + p)]);
-    high = wave_max(high);
-    const float shift = high == -INFINITY ? 0.f : high;
+    // A part (of up to 64) a lane: its weight, which the others take from there.  Up to eight parts' outputs are asked for together (8
+    // parts of 208 nodes, 32 heads of 64: 4.5 us, one after the other 6.3).
+    const bool has = lane < a.parts;
+    const float m = has ? a.ws_ml[2 * (at + lane)] : -INFINITY, l = has ? a.ws_ml[2 * (at + lane) + 1] : 0.f;
+    const float high = wave_max(m), weight = __builtin_amdgcn_exp2f(m - (high == -INFINITY ? 0.f : high));
+    const float sum = wave_sum(weight * l);
     constexpr int PER = (HD + 63) / 64;
-    float sum = 0.f, o[PER] = {};
-    for (int p = 0; p < a.parts; ++p) {
-        const float w = __builtin_amdgcn_exp2f(a.ws_ml[2 * (at + p)] - shift);
-        sum = fmaf(w, a.ws_ml[2 * (at + p) + 1], sum);
+    float o[PER] = {};
+    auto add = [&](auto together, int p0) {
+        constexpr int N = decltype(together)::value;
+        float from[N][PER];
 #pragma unroll
-        for (int e = 0; e < PER; ++e)
-            if (lane + 64 * e < HD) o[e] = fmaf(w, a.ws_o[(at + p) * HD + lane + 64 * e], o[e]);
+        for (int p = 0; p < N; ++p)
+#pragma unroll
+            for (int e = 0; e < PER; ++e) from[p][e] = a.ws_o[(at + min(p0 + p, a.parts - 1)) * HD + min(lane + 64 * e, HD - 1)];
+#pragma unroll
+        for (int p = 0; p < N; ++p) {
+            const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), p0 + p));
+#pragma unroll
+            for (int e = 0; e < PER; ++e) o[e] = p0 + p < a.parts ? fmaf(w, from[p][e], o[e]) : o[e];
+        }
+    };
+    for (int p0 = 0; p0 < a.parts;) {
+        if (a.parts - p0 <= 2) {
+            add(std::integral_constant<int, 2>{}, p0);
+            p0 += 2;
+        } else {
+            add(std::integral_constant<int, 8>{}, p0);
+            p0 += 8;
+        }
     }
     T* to = static_cast<T*>(a.out) + (static_cast<size_t>(first + node) * a.heads + head) * HD;
 #pragma unroll
@@ -849,8 +867,8 @@ extern "C" int celeg_tree_attention_fast_ok(int head_dim, int page_tokens) {
 // 16 heads of 64 on 8, behind 700: 9.2 us, in 3 parts 9.8, and a launch less for the host; behind 1,500: 13.3 and 10.6).
 //   More: 256 workgroups, one a compute unit, each wavefront (each workgroup that stages: two) with a round at least: a second one beside it
 // gains less than its part costs to join (4 trees of 8 behind 6,000, 32 heads of 64 on 8: 20.0 us, of 512 workgroups 22.9; heads
-// of 128 29.7 and 34.9; 4 of 26 behind 2,500, staged: 16.7 and 21.3).  Staged rounds in long parts, more than 16 of them, gain more (8
-// of 26 behind 16,000: 64 us, of 256 workgroups 80; behind 2,500 25 and 25).
+// of 128 29.7 and 34.9; 4 of 26 behind 2,500, staged: 16.7 and 21.3).  Staged rounds in long parts, more than 16 of them (40 of wider
+// heads), gain more (8 of 26 behind 16,000: 74 us, of 256 workgroups 85, heads of 128 123 and 135; behind 2,500 26 and 26, 36 and 34).
 extern "C" int celeg_tree_attention_parts(int dtype, int head_dim, int requests, int kv_heads, int group, int max_nodes, int max_context) {
     const int rows = max_nodes * group;
     const TreeForm form = tree_form(dtype, head_dim, rows);
@@ -858,7 +876,7 @@ extern "C" int celeg_tree_attention_parts(int dtype, int head_dim, int requests,
     const long long rounds = (static_cast<long long>(max_context) + max_nodes + form.keys - 1) / form.keys;
     if (rounds <= (form.staged ? 4 : 12)) return 1;
     long long parts = (256 + groups - 1) / groups;
-    if (form.staged && form.resident > 1 && rounds > 16 * parts) parts = (256 * form.resident + groups - 1) / groups;
+    if (form.staged && form.resident > 1 && rounds > (head_dim > 64 ? 40 : 16) * parts) parts = (256 * form.resident + groups - 1) / groups;
     return static_cast<int>(std::max(1LL, std::min({parts, form.staged ? (rounds + 1) / 2 : (rounds + 3) / 4, 64LL})));
 }
 
