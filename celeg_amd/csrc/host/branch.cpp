@@ -105,7 +105,8 @@ static int tree_parts(const TreeAttention& a, const KVView& kv) {
     const long long page_bytes = static_cast<long long>(kv.n_layers) * kv.kv_heads * kv.page_tokens * kv.head_dim * static_cast<long long>(dtype_size(kv.dtype));
     if (low % 16 || page_bytes >= (1LL << 31) || !celeg_tree_attention_fast_ok(kv.head_dim, kv.page_tokens)) return 0;
     const long long room = static_cast<long long>(kv.table_stride) * kv.page_tokens;
-    const int context = static_cast<int>(a.max_context > 0 ? std::min<long long>(a.max_context, room) : room);
+    int context = static_cast<int>(a.max_context > 0 ? std::min<long long>(a.max_context, room) : room);
+    if (a.window > 0) context = std::min(context, a.window);        // (nothing before it is read)
     return celeg_tree_attention_parts(static_cast<int>(kv.dtype), kv.head_dim, a.requests, kv.kv_heads, a.heads / kv.kv_heads, a.max_nodes, context);
 }
 

@@ -420,8 +420,14 @@ __global__ __launch_bounds__(256, 2) void tree_few_kernel(const TreeArgs a) {
     int node_of[RT];
     tree_queries<T, HD, RT>(a, w, kvh, j0, q, node_of);
     const int n0 = j0 / a.group, n1 = min(j0 + ROWS - 1, w.rows - 1) / a.group;      // the block's nodes
-    tree_ways<256>(a, w, n0, n1, up, words_of, low_of);
     const TreeRounds rounds(a, w, part, KEYS);
+    // the pages of a round, a lane each; asked for a round ahead (the first one's before the ways up the tree are gone)
+    auto pages_of = [&](int round) {
+        const int base = round * KEYS, last = (min(base + KEYS, w.end) - 1) >> a.page_shift;
+        return round <= rounds.r_end ? w.pages[min((base >> a.page_shift) + lane, last)] : 0;
+    };
+    int next_page = pages_of(rounds.r_begin + wave);
+    tree_ways<256>(a, w, n0, n1, up, words_of, low_of);
     float m[RT], l[RT];
     tree_f4 o[RT][DT];
 #pragma unroll
@@ -434,7 +440,7 @@ __global__ __launch_bounds__(256, 2) void tree_few_kernel(const TreeArgs a) {
     for (int round = rounds.r_begin + (tid >> 6); round <= rounds.r_end; round += 4) {
         const int base = round * KEYS, top = min(base + KEYS, w.end) - 1;
         const int first_page = base >> a.page_shift, last_page = top >> a.page_shift;
-        int page = w.pages[min(first_page + lane, last_page)];
+        int page = next_page;
         const bool there = page >= 0 && page < a.n_pages;
         const bool all_there = __ballot(!there) == 0ull;
         page = there ? page : 0;
@@ -454,6 +460,7 @@ __global__ __launch_bounds__(256, 2) void tree_few_kernel(const TreeArgs a) {
             for (int dt = 0; dt < DT; ++dt)
                 v[dt][g] = *reinterpret_cast<const Frag*>(from + (static_cast<size_t>(16 * dt + c) << a.page_shift));
         }
+        next_page = pages_of(round + 4);
         if (base >= rounds.plain && base + KEYS <= w.start && all_there) {
             tree_f4 s[RT][TILES];
 #pragma unroll
