@@ -256,8 +256,8 @@ const char* celeg_reference_call(const char* op, const char* args_json);
  * several threads, on several streams, or recorded into graphs, are independent as far as their memory is.  Wrong
  * arguments are refused with CELEG_INVALID_ARGUMENT before anything is launched (without a GPU too).  Structs carry their size
  * in struct_size.  dtype: 0 float32, 1 bfloat16.  A call with nothing to do (no rows, no requests, no pages) is CELEG_OK.
- * Workspaces: 16-byte aligned device memory of the size that the *_workspace function gives for the same arguments (it does not
- * look at addresses of data); they hold nothing between calls, and two calls that may run at the same time need one each. */
+ * Workspaces: 16-byte aligned device memory of the size that the *_workspace function gives for the same arguments (addresses of
+ * data need not be there yet); they hold nothing between calls, and two calls that may run at the same time need one each. */
 
 /* All layers of one group of pages: k [n_pages, n_layers, kv_heads, page_tokens, head_dim], v [n_pages, n_layers, kv_heads,
  * v_head_dim, page_tokens] (null with v_head_dim 0: keys only), table [table_rows, table_stride]: row s names the pages of slot s.
