@@ -277,7 +277,8 @@ def _judge(lm, prompt, top, portion) -> None:
               f"entropy={judged.entropy[i]:.4f}" + (f" top={best}" if best else ""), file=sys.stderr)
     if len(prompt) > 1:
         mean = judged.logprobs.double().mean().item()
-        print(f"prompt.mean_logprob={mean:.6f}\nprompt.perplexity={math.exp(-mean):.6f}", file=sys.stderr)
+        perplexity = math.inf if mean < -700 else math.exp(-mean)       # (more than a double holds)
+        print(f"prompt.mean_logprob={mean:.6f}\nprompt.perplexity={perplexity:.6f}", file=sys.stderr)
 
 
 def _reports(args, engine, request_id=None) -> None:

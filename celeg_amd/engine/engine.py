@@ -213,6 +213,8 @@ class LoadedModel:
         ``tokens[i + 1]`` (one row fewer than tokens), with the ``top`` best tokens there.  Takes a slot of the
         cache for the time of the call; in portions of at most ``portion`` tokens (the step's largest)."""
         tokens = [int(t) for t in tokens]
+        if portion is not None and portion < 1:
+            raise ValueError("score: a portion must have at least one token")
         portion = min(portion or self.runner.max_batched_tokens, self.runner.max_batched_tokens)
         slot = self.cache.open()
         if slot is None:

@@ -85,6 +85,42 @@ def test_every_path_of_a_tree_is_as_if_it_were_alone(attention_folders, name, dt
     lm.close()
 
 
+@pytest.mark.parametrize("dtype,stored", DTYPES)
+@pytest.mark.parametrize("wanted", ["few", "all"])
+def test_steps_of_many_rows(tmp_path, dtype, stored, wanted):
+    """More rows than the kernels for few of them take, in a model wide enough for the tiled products; with few wanted rows the last
+    layer goes on with those alone."""
+    from celeg_amd.engine import StepEntry
+    from celeg_amd.weights import write_random_model
+    cfg, seed = TINY["D"]
+    cfg = dict(cfg, hidden_size=256, num_attention_heads=4, num_key_value_heads=2, layer_types=["full_attention"] * cfg["num_hidden_layers"])
+    folder = write_random_model(cfg, str(tmp_path), seed=seed, dtype=stored, std=WEIGHT_STD)
+    cfg, W = plain.load_model_folder(folder)
+    V = cfg["vocab_size"]
+    lm = load(folder, dtype, max_batched_tokens=320)
+    assert lm.takes_trees
+    gen = torch.Generator().manual_seed(8)
+    entries, looked = [], []
+    for context, n, branches in ((45, 150, True), (0, 83, True), (130, 70, False)):
+        slot = lm.cache.open()
+        seq = random_tokens(V, context, seed=context)
+        if seq:
+            feed(lm, slot, seq, portion=320)
+        parents = [int(torch.randint(max(-1, i - 6), i, (1,), generator=gen)) for i in range(n)] if branches else []
+        tokens = random_tokens(V, n, seed=n)
+        assert lm.cache.prepare(slot, context, n)
+        nodes = [0, n // 2, n - 1]
+        entries.append(StepEntry(slot, context, tokens, nodes if wanted == "few" else range(n), parents))
+        for i in nodes:
+            looked.append((len(looked) if wanted == "few" else sum(len(e.want) for e in entries[:-1]) + i, seq,
+                           [tokens[j] for j in (way(parents, i) if branches else range(i + 1))]))
+    got = lm.runner.step(entries)
+    assert lm.paths()["attention_trees"] == cfg["num_hidden_layers"]
+    for row, seq, path in looked:
+        assert_close(got[row], plain.model_logits(cfg, W, seq + path)[-1], dtype, f"row {row}: {len(path)} tokens behind {len(seq)}")
+    lm.close()
+
+
 @pytest.mark.parametrize("name", ["D", "B"])
 @pytest.mark.parametrize("dtype,stored", DTYPES)
 def test_the_accepted_path_is_kept_and_goes_on(attention_folders, name, dtype, stored):
@@ -184,6 +220,9 @@ def test_a_sequence_is_scored(model_folders, name, dtype, stored):
         assert torch.equal(got.top_ids[:, 0].long(), want.argmax(1))
         assert torch.equal(got.ranks[:, 0].long(), (want > want.gather(1, at[:, None])).sum(1))
     assert lm.cache.n_free_slots == 4
+    for portion in (0, -3):
+        with pytest.raises(ValueError, match="portion"):
+            lm.score(tokens, portion=portion)
     assert lm.score([3]).logprobs.shape == (0, 1) and lm.score([], top=2).top_ids.shape == (0, 2)
     # the device's answers are those of the logits themselves
     from celeg_amd.engine import StepEntry
@@ -196,6 +235,92 @@ def test_a_sequence_is_scored(model_folders, name, dtype, stored):
     assert judged.logprobs[1, 1].isnan() and judged.ranks[1, 1] == -1
     assert torch.equal(judged.top_ids.long(), rows.topk(3).indices)
     assert lm.runner.logprobs([StepEntry(slot, 0, tokens[:6])]).logprobs.shape == (0, 0)
+    lm.close()
+
+
+# ---------------------------------------------------------------- layers with and without windows
+WINDOWS = (20, None, 7)
+
+
+def windowed_folder(path, dtype):
+    """A model of three attention layers of which two see the last tokens alone, so that their pages are given back early."""
+    from celeg_amd.config import LayerSpec, ModelSpec, PartSpec, RunStep, register_architecture, registered_architectures
+    from celeg_amd.weights import write_random_model
+
+    def build_spec(cfg, shapes):
+        H = cfg["width"]
+        norm = lambda name: PartSpec("rmsnorm", {"width": H, "eps": 1e-5}, {"weight": name})
+        layers = []
+        for i, window in enumerate(WINDOWS):
+            p = f"blocks.{i}."
+            layers.append(LayerSpec(
+                PartSpec("gqa_attention", {"width": H, "heads": 4, "kv_heads": 2, "head_dim": 16, "qk_norm": False, "window": window,
+                                           "position": PartSpec("rope", {"theta": 100.0, "head_dim": 16})},
+                         {"q_proj": p + "att.q", "k_proj": p + "att.k", "v_proj": p + "att.v", "out_proj": p + "att.o"}),
+                norm(p + "n1"), PartSpec("swiglu", {"width": H, "ff": 2 * H}, {"gate": p + "ff.g", "up": p + "ff.u", "down": p + "ff.d"}),
+                norm(p + "n2")))
+        return ModelSpec("WindowedForCausalLM", cfg["vocab"], H, 256, PartSpec("embedding", {"vocab": cfg["vocab"], "width": H}, {"table": "emb"}),
+                         tuple(layers), tuple(RunStep(i) for i in range(len(layers))), norm("final"),
+                         PartSpec("tied_head", {"vocab": cfg["vocab"], "width": H}))
+
+    if "WindowedForCausalLM" not in registered_architectures():
+        register_architecture("WindowedForCausalLM", build_spec)
+    return write_random_model({"architectures": ["WindowedForCausalLM"], "width": 64, "vocab": 91}, path, seed=12, dtype=dtype, std=WEIGHT_STD)
+
+
+def windowed_logits(W, tokens):
+    h = plain.embedding(W["emb"], tokens)
+    T = len(tokens)
+    for i, window in enumerate(WINDOWS):
+        p = f"blocks.{i}."
+        n = plain.rmsnorm(h, W[p + "n1"], 1e-5)
+        cos, sin = plain.rope_cos_sin(range(T), 100.0, 16)
+        q, k, v = (plain.linear(n, W[p + "att." + x]).reshape(T, -1, 16) for x in "qkv")
+        o = plain.causal_attention(plain.rope_apply(q, cos, sin), plain.rope_apply(k, cos, sin), v, window=window)
+        h = h + plain.linear(o.reshape(T, -1), W[p + "att.o"])
+        h = h + plain.swiglu_ffn(plain.rmsnorm(h, W[p + "n2"], 1e-5), W[p + "ff.g"], W[p + "ff.u"], W[p + "ff.d"])
+    return plain.linear(plain.rmsnorm(h, W["final"], 1e-5), W["emb"])[-1]
+
+
+@pytest.mark.parametrize("dtype,stored", DTYPES)
+def test_trees_keeps_and_forks_with_windows(tmp_path, dtype, stored):
+    from celeg_amd.engine import StepEntry
+    folder = windowed_folder(str(tmp_path / "windowed"), stored)
+    _, W = plain.load_model_folder(folder)
+    lm = load(folder, dtype, page_tokens=4)
+    assert lm.takes_trees
+    slot = lm.cache.open()
+    seqs = {slot: random_tokens(91, 53, seed=1)}
+    feed(lm, slot, seqs[slot])
+    for turn, leaf in enumerate((10, 7, 9, 5)):
+        if turn == 2:
+            seqs[lm.cache.fork(slot, len(seqs[slot]))] = list(seqs[slot])
+            lm.cache.check()
+        entries = []
+        for s, seq in seqs.items():
+            tokens = random_tokens(91, len(TREE), seed=10 * turn + s)
+            assert lm.cache.prepare(s, len(seq), len(TREE))
+            entries.append(StepEntry(s, len(seq), tokens, range(len(TREE)), TREE))
+        got = lm.runner.step(entries)
+        for j, e in enumerate(entries):
+            for i in range(len(TREE)):
+                assert_close(got[j * len(TREE) + i], windowed_logits(W, seqs[e.slot] + [e.tokens[x] for x in way(TREE, i)]), dtype,
+                             f"turn {turn}, slot {e.slot}, node {i}")
+            path = way(TREE, leaf)
+            lm.cache.keep(e.slot, e.start_pos, [e.start_pos + i for i in path])
+            lm.cache.check()
+            seqs[e.slot] = seqs[e.slot] + [e.tokens[i] for i in path]
+    for s, seq in seqs.items():                         # decoding behind what was kept
+        assert lm.cache.prepare(s, len(seq), 1)
+        got = lm.runner.step([StepEntry(s, len(seq), [5], [0])])
+        assert_close(got[0], windowed_logits(W, seq + [5]), dtype, f"slot {s}")
+    # back to before what the windows have given back: refused, as the keys there are gone
+    lm.cache.keep(slot, 12)
+    assert lm.cache.prepare(slot, 12, 1)
+    with pytest.raises(ValueError, match="cover"):
+        lm.runner.step([StepEntry(slot, 12, [1], [0])])
+    lm.cache.close(slot)
+    lm.cache.check()
     lm.close()
 
 
