@@ -46,7 +46,7 @@ def build_parser() -> argparse.ArgumentParser:
                     help="write the logits after the prompt as raw 32-bit floats")
     ap.add_argument("--print-top", type=int, default=0, metavar="N")
     ap.add_argument("--prompt-logprobs", type=int, default=None, metavar="N",
-                    help="judge the prompt itself: for every token behind the first its log probability and rank and the N (up to 128) "
+                    help="score the prompt itself: for every token behind the first its log probability and rank and the N (up to 128) "
                          "most likely tokens in its place, and the perplexity, on stderr")
     ap.add_argument("--tokens-only", action="store_true", help="print the prompt's ids and exit")
     ap.add_argument("--runtime-tokens", action="store_true",
@@ -229,7 +229,7 @@ def run(args) -> int:
         return 0
 
     if args.prompt_logprobs is not None:
-        _judge(lm, prompt, min(args.prompt_logprobs, lm.native.logit_width), min(args.prefill_chunk, budget))
+        _score_prompt(lm, prompt, min(args.prompt_logprobs, lm.native.logit_width), min(args.prefill_chunk, budget))
 
     generation = GenerationConfig(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
                                   repetition_penalty=args.repetition_penalty, seed=args.seed)
@@ -268,7 +268,7 @@ def run(args) -> int:
     return 0
 
 
-def _judge(lm, prompt, top, portion) -> None:
+def _score_prompt(lm, prompt, top, portion) -> None:
     """--prompt-logprobs: a line for every token behind the first, then the perplexity."""
     judged = lm.score(prompt, top=top, portion=portion)
     for i, target in enumerate(prompt[1:]):

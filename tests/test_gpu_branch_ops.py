@@ -527,7 +527,7 @@ def test_draft_judge_keep_and_go_on():
     children = ints([[1, 2], [3, 4], [5, -1], [-1, -1], [6, 7], [-1, -1], [8, -1], [-1, -1], [-1, -1]])       # (a draft's token is its index here)
     judged = ops.token_logprobs(out[:9] @ head, children, top=3)
     assert torch.equal(judged.logprobs.isnan(), children < 0)
-    # the path that the judge likes best, a node at a time
+    # the path that the scoring model likes best, a node at a time
     path, at = [0], 0
     while (children[at] >= 0).any():
         at = int(children[at][judged.logprobs[at].nan_to_num(-math.inf).argmax()])
