@@ -32,7 +32,7 @@ typedef float lp_f4 __attribute__((ext_vector_type(4)));
 typedef unsigned int lp_u4 __attribute__((ext_vector_type(4)));
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
-constexpr float LP_FITS = 1e38f;          // below it a logit times log2(e) is a number
+constexpr float LP_FITS = 16777216.f;     // below it m log2(e) is rounded by at most 1
 
 // 16 bytes of logits as they lie in memory
 template <typename T> struct LogitGroup;
@@ -75,25 +75,17 @@ __device__ __forceinline__ float best_logit(unsigned long long packed) {
     return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
 }
 
-// x's distance from the largest, in powers of two, as the sums take it
-__device__ __forceinline__ float logit_distance(float x, float m) { return fabsf(m) < LP_FITS ? fmaf(x, LOG2E, -(m * LOG2E)) : (x - m) * LOG2E; }
+// What the rounding of m log2(e), from which the sums take their distances, left out of it: the same for every logit, so that 2^-this
+// brings a sum against the rounded product to one against m itself.  Below LP_FITS it is no more than 1; from there on m is taken off
+// first, and nothing is left out (a row of 1,000 logits of 1e10 is off by 440 powers of two otherwise).
+__device__ __forceinline__ float left_out(float m) { return fabsf(m) < LP_FITS ? fmaf(m, LOG2E, -(m * LOG2E)) : 0.f; }
 
-__device__ __forceinline__ float logprob_of(float x, float m, float log2_sum) {
-    const float d = logit_distance(x, m);
-    return d == -INFINITY ? (x - m) - log2_sum * LN2 : (d - log2_sum) * LN2;       // (what is far below may fit in nats alone)
-}
+// (log2_sum: of the exponentials against m itself)
+__device__ __forceinline__ float logprob_of(float x, float m, float log2_sum) { return (x - m) - log2_sum * LN2; }
 
 // Of n packed logits in `list` (all different), the `top` largest in falling order: put(place, packed).  All threads call it, behind a
 // barrier; there is one more in it.  They are counted against one another eight at a time, whose reads are under way together (the list
 // has room for eight more, which are made 0): one at a time 128 best took twice as long as all the rest.
-// The same of a part's largest, as the part has it: its sums are against the rounded product.
-__device__ __forceinline__ float part_distance(float part, float m) {
-    if (!(fabsf(part) < LP_FITS && fabsf(m) < LP_FITS)) return (part - m) * LOG2E;
-    float of_part = part * LOG2E;
-    asm volatile("" : "+v"(of_part));        // (rounded, as the part's sums have it: not taken into the subtraction)
-    return of_part - m * LOG2E;
-}
-
 template <int THREADS, typename F>
 __device__ __forceinline__ void sorted_best(unsigned long long* list, int n, int top, F put) {
     typedef unsigned long long two __attribute__((ext_vector_type(2)));
@@ -287,7 +279,7 @@ __global__ __launch_bounds__(THREADS, 1024 / THREADS) void logprobs_part_kernel(
         if (lane == 0) bounds[wave] = least;
     }
     // ---- the sums, of d = x log2(e) - m log2(e).  Below -2000 the exponential is 0 in any case, and 0 times -2000 is no NaN.
-    // Where m log2(e) would not fit (a row of the type's lowest value), the maximum is taken off first.
+    // Where m log2(e) is rounded by more than 1 (a row masked throughout by -1e10), the maximum is taken off first.
     const float m = high == -INFINITY ? 0.f : high;
     float sum = 0.f, moment = 0.f;
     auto add = [&](float d) {
@@ -389,8 +381,8 @@ __global__ __launch_bounds__(THREADS, 1024 / THREADS) void logprobs_part_kernel(
         return;
     }
     const bool none = bad || high == INFINITY || high == -INFINITY;
-    const float log2_sum = none ? NAN : __builtin_amdgcn_logf(sum);
-    if (tid == 0 && out.entropy) out.entropy[row] = (log2_sum - moment / sum) * LN2;
+    if (tid == 0 && out.entropy) out.entropy[row] = none ? NAN : (__builtin_amdgcn_logf(sum) - moment / sum) * LN2;
+    const float log2_sum = none ? NAN : __builtin_amdgcn_logf(sum) - left_out(m);
     if (tid < per_row) {
         const int t = tokens[row * per_row + tid];
         const bool valid = t >= 0 && t < vocab;
@@ -445,7 +437,8 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_join_kernel(
     float sum = 0.f, moment = 0.f;
     for (int p = tid; p < parts; p += LP_THREADS) {
         const float4 s = stats[p];
-        const float d = fmaxf(part_distance(s.x, m), -2000.f), w = __builtin_amdgcn_exp2f(d);
+        // (the part's sums are against its own largest as the part has it)
+        const float d = fmaxf((s.x - m) * LOG2E - left_out(s.x), -2000.f), w = __builtin_amdgcn_exp2f(d);
         sum = fmaf(w, s.y, sum);
         moment = fmaf(w, fmaf(d, s.y, s.z), moment);
     }
