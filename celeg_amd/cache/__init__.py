@@ -116,9 +116,14 @@ class CacheManager(_Host):
     def covers(self, slot: int, start_pos: int, n_new: int) -> bool:
         return self._call("covers", slot, start_pos, n_new)
 
+    def stepped(self, slot: int, length: int) -> None:
+        """A step has left the state of ``slot`` behind its first ``length`` tokens (the model's runner says so by itself)."""
+        self._call("stepped", slot, length)
+
     def fork(self, slot: int, length: int) -> Optional[int]:
         """A request that goes on from the first ``length`` tokens of ``slot``: their pages are shared until one of the
-        two prepares to write to one.  None: every slot is taken."""
+        two prepares to write to one.  With state beside keys and values, ``length`` has to be what the request has been
+        stepped to.  None: every slot is taken."""
         other = self._call("fork", slot, length)
         return None if other < 0 else other
 

@@ -172,6 +172,7 @@ CacheManager::CacheManager(CacheLayout layout_, int page_tokens_, std::vector<in
     slot_bytes = offset;
     if (on_device_) state_buffer_ = DeviceBuffer(static_cast<size_t>(max_requests + 1) * std::max<size_t>(offset, 16), true);
     for (int s = max_requests - 1; s >= 0; --s) free_slots_.push_back(s);
+    stepped_.assign(static_cast<size_t>(max_requests), 0);
 }
 
 std::vector<int> CacheManager::open_slots() const {
@@ -185,6 +186,7 @@ int CacheManager::open() {
     const int slot = free_slots_.back();
     free_slots_.pop_back();
     open_[slot] = 0;
+    stepped(slot, 0);
     if (slot_bytes && on_device_)
         CELEG_HIP(hipMemsetAsync(static_cast<char*>(state_buffer_.ptr()) + static_cast<size_t>(slot) * slot_bytes, 0,
                                  slot_bytes, stream_));
@@ -335,6 +337,9 @@ int CacheManager::fork(int slot, int length) {
     if (length < 0 || length > open_.at(slot))
         throw PageError("fork: slot " + std::to_string(slot) + " has pages for " + std::to_string(open_.at(slot)) + " tokens, not " +
                         std::to_string(length));
+    if (slot_bytes && length != stepped_[static_cast<size_t>(slot)])
+        throw PageError("fork: the state of slot " + std::to_string(slot) + " stands behind " + std::to_string(stepped_[static_cast<size_t>(slot)]) +
+                        " tokens, not " + std::to_string(length) + ", and cannot go back");
     const int other = open();
     if (other < 0) return -1;
     const int count = (length + page_tokens - 1) / page_tokens;
@@ -357,6 +362,7 @@ int CacheManager::fork(int slot, int length) {
                                  hipMemcpyDeviceToDevice, stream_));
     }
     open_[other] = length;
+    stepped(other, length);
     return other;
 }
 

@@ -137,10 +137,13 @@ public:
     bool prepare(int slot, int start_pos, int n_new);
     // whether the request's pages cover these positions, and none of those is shared with another request
     bool covers(int slot, int start_pos, int n_new) const;
-    // A request that goes on from the first `length` tokens of an open one, with its state as it stands.  The pages that
-    // hold them are shared until either request is about to write to one: prepare() then gives that one a copy of its own.
+    // A request that goes on from the first `length` tokens of an open one.  The pages that hold them are shared until either
+    // request is about to write to one: prepare() then gives that one a copy of its own.  State beside keys and values is
+    // copied as it stands, so where there is any, `length` has to be the tokens that the request has been stepped to.
     // -1: every slot is taken.
     int fork(int slot, int length);
+    // a step has left the request's state behind its first `length` tokens
+    void stepped(int slot, int length) { stepped_[static_cast<size_t>(slot)] = length; }
     // forgets the tokens from `length` on: pages that hold none of the others are given back
     void truncate(int slot, int length);
     int tokens(int slot) const { return open_.count(slot) ? open_.at(slot) : 0; }      // that the request has been given pages for
@@ -195,6 +198,7 @@ private:
     hipStream_t stream_;
     std::vector<int> free_slots_;
     std::map<int, int> open_;       // slot -> tokens covered by pages so far
+    std::vector<int> stepped_;      // per slot: tokens that its state stands behind
 };
 
 }  // namespace celeg

@@ -95,6 +95,12 @@ Json call(HostObject& o, const std::string& method, const Json& a) {
         if (method == "pages_needed") return Json::array_of(c.pages_needed(static_cast<int>(a[0].as_int()), static_cast<int>(a[1].as_int()), static_cast<int>(a[2].as_int())));
         if (method == "check") { c.check(); return Json(true); }
         if (method == "fork") return Json(c.fork(static_cast<int>(a[0].as_int()), static_cast<int>(a[1].as_int())));
+        if (method == "stepped") {
+            const int slot = static_cast<int>(a[0].as_int());
+            if (slot < 0 || slot >= c.max_requests) throw PageError("slot " + std::to_string(slot) + " does not exist");
+            c.stepped(slot, static_cast<int>(a[1].as_int()));
+            return Json(true);
+        }
         if (method == "truncate") { c.truncate(static_cast<int>(a[0].as_int()), static_cast<int>(a[1].as_int())); return Json(true); }
         if (method == "holds") return Json(c.holds(static_cast<int>(a[0].as_int()), static_cast<int>(a[1].as_int()), static_cast<int>(a[2].as_int())));
         if (method == "pages_held") {

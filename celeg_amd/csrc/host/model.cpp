@@ -455,6 +455,12 @@ void ModelRunner::begin_step(const StepBatch& batch) {
 
 Tensor ModelRunner::step(const std::vector<StepEntry>& entries) {
     validate(entries);
+    const Tensor logits = run_step(entries);
+    for (const StepEntry& e : entries) cache.stepped(e.slot, e.start_pos + static_cast<int>(e.tokens.size()));
+    return logits;
+}
+
+Tensor ModelRunner::run_step(const std::vector<StepEntry>& entries) {
     for (const StepEntry& e : entries)
         if (!e.parents.empty()) return step_of_trees(entries);
     if (graph_applies(entries)) return step_from_graph(entries);

@@ -111,6 +111,7 @@ private:
     bool graph_applies(const std::vector<StepEntry>& entries) const;
     int context_bound(const std::vector<StepEntry>& entries, int bucket) const;
     std::map<int, std::vector<int>> short_contexts_;      // by the bucket of a recorded step
+    Tensor run_step(const std::vector<StepEntry>& entries);
     Tensor step_of_trees(const std::vector<StepEntry>& entries);
     Tensor step_from_graph(const std::vector<StepEntry>& entries);
     Captured& capture(int bucket, const std::vector<int>& caps, int bound);

@@ -180,7 +180,8 @@ celeg_status celeg_model_step_logprobs(celeg_model* model, int32_t n_entries, co
                                        const int32_t* want, const int32_t* targets, int32_t per_row, int32_t top, float* logprobs,
                                        int32_t* ranks, float* entropy, int32_t* top_ids, float* top_logprobs);
 /* A slot for a request that goes on from the first `length` tokens of another (of those celeg_model_prepare has given it pages
- * for), its state beside keys and values as it stands.  Pages are shared; celeg_model_prepare gives whoever writes to a shared one
+ * for).  State beside keys and values is copied as it stands: a model that keeps any refuses a `length` other than the tokens
+ * that the request has been stepped to.  Pages are shared; celeg_model_prepare gives whoever writes to a shared one
  * a copy of its own (both have to call it before their next step).  *new_slot -1: every slot is taken. */
 celeg_status celeg_model_fork_slot(celeg_model* model, int32_t slot, int32_t length, int32_t* new_slot);
 /* Of a slot's tokens from place `start` on, those at the n `places` (rising) stay and come to stand at start, start + 1, ..; the rest is

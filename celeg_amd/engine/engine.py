@@ -121,8 +121,9 @@ class _CacheFacade:
         return self._m.prepare(slot, start_pos, n_new)
 
     def fork(self, slot: int, length: int) -> Optional[int]:
-        """A slot that goes on from the first ``length`` tokens of another, with its state as it stands; the pages are shared
-        until ``prepare`` says that one of the two writes to one.  None: every slot is taken."""
+        """A slot that goes on from the first ``length`` tokens of another; the pages are shared until ``prepare`` says that one
+        of the two writes to one.  A model that keeps state can fork a request only where it stands (ValueError for a
+        ``length`` other than the tokens stepped).  None: every slot is taken."""
         try:
             return self._m.fork_slot(slot, length)
         except native.NativeError as err:
