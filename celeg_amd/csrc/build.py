@@ -206,10 +206,12 @@ SANITIZE_FLAGS = ["-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fsanitiz
                   "-fno-omit-frame-pointer", "-g1"]
 
 
-def build_sanitized(out_dir: str, verbose: bool = False) -> str:
+def build_sanitized(out_dir: str, verbose: bool = False, hip_stand_in: Optional[str] = None) -> str:
     """The library with its HOST code under AddressSanitizer and UndefinedBehaviorSanitizer (the
     kernels' objects are the ordinary ones; device code is never instrumented), linked into
-    ``out_dir``: what the tests of the host's memory safety run, on the CPU.  Returns its path."""
+    ``out_dir``: what the tests of the host's memory safety run, on the CPU.  ``hip_stand_in``: a C++ source
+    whose functions take the place of the HIP runtime's, so that the paths that need a device run without
+    one.  Returns the library's path."""
     with _lock:
         lib_dir = _writable_lib_dir()
         os.makedirs(os.path.join(out_dir, "obj"), exist_ok=True)
@@ -224,8 +226,13 @@ def build_sanitized(out_dir: str, verbose: bool = False) -> str:
             return obj
         with ThreadPoolExecutor(max_workers=max(1, min(8, os.cpu_count() or 1))) as pool:
             hosts = list(pool.map(sanitized, host_sources()))
-        final = os.path.join(out_dir, LIBRARY + "-sanitized.so")
-        _run([_hipcc()] + kernels + hosts + LINK_FLAGS + SANITIZE_FLAGS[:4] + ["-o", final], "linking", out_dir, verbose)
+        final = os.path.join(out_dir, LIBRARY + ("-sanitized.so" if hip_stand_in is None else "-sanitized-stand-in.so"))
+        runtime = []
+        if hip_stand_in is not None:
+            runtime = [os.path.join(out_dir, "obj", "hip_stand_in.o"), "-no-hip-rt"]
+            _run([_hipcc(), "-std=c++17", "-O1", "-g1", "-fPIC", "-x", "hip", f"--offload-arch={ARCH}"] + SANITIZE_FLAGS + ["-c", hip_stand_in, "-o", runtime[0]],
+                 "compiling the stand-in of the HIP runtime", out_dir, verbose)
+        _run([_hipcc()] + kernels + hosts + runtime + LINK_FLAGS + SANITIZE_FLAGS[:4] + ["-o", final], "linking", out_dir, verbose)
         return final
 
 

@@ -315,11 +315,17 @@ bool CacheManager::unshare(int slot, int start_pos, int n) {
         for (int idx : shared[gi]) lists.push_back(pages[static_cast<size_t>(idx)]);
         lists.insert(lists.end(), fresh.begin(), fresh.end());
         if (on_device_) {
-            const size_t bytes = lists.size() * sizeof(int);
-            if (copy_list_.bytes() < bytes) copy_list_ = DeviceBuffer(std::max<size_t>(bytes, 1024));
-            CELEG_HIP(hipMemcpyAsync(copy_list_.ptr(), lists.data(), bytes, hipMemcpyHostToDevice, stream_));
-            copy_pages(group_view(static_cast<int>(gi)), copy_list_.as<int>(), copy_list_.as<int>() + count, count, stream_);
-            CELEG_HIP(hipStreamSynchronize(stream_));      // (the lists go away)
+            try {
+                const size_t bytes = lists.size() * sizeof(int);
+                if (copy_list_.bytes() < bytes) copy_list_ = DeviceBuffer(std::max<size_t>(bytes, 1024));
+                CELEG_HIP(hipMemcpyAsync(copy_list_.ptr(), lists.data(), bytes, hipMemcpyHostToDevice, stream_));
+                copy_pages(group_view(static_cast<int>(gi)), copy_list_.as<int>(), copy_list_.as<int>() + count, count, stream_);
+                CELEG_HIP(hipStreamSynchronize(stream_));      // (the lists go away)
+            } catch (...) {
+                (void)hipStreamSynchronize(stream_);
+                g.pool.release(fresh);       // (nobody holds them yet)
+                throw;
+            }
         }
         for (int i = 0; i < count; ++i) {
             const int idx = shared[gi][static_cast<size_t>(i)];
