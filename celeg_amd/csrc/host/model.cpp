@@ -548,8 +548,13 @@ void ModelRunner::keep(int slot, int start, const std::vector<int>& places) {
         if (!cache.unshare(slot, start + first, n - first)) throw StepError("keep: no free page for what is shared with another request");
         // the device's block tables as the host's are
         auto updates = cache.drain_table_updates();
-        for (size_t g = 0; g < updates.size(); ++g)
-            if (!updates[g].empty()) ship_table_updates(static_cast<int>(g), updates[g]);
+        try {
+            for (size_t g = 0; g < updates.size(); ++g)
+                if (!updates[g].empty()) ship_table_updates(static_cast<int>(g), updates[g]);
+        } catch (...) {
+            cache.requeue_table_updates(updates);        // (the next step or call brings them)
+            throw;
+        }
         std::vector<int> lists{slot, 0, n - first, start + first};
         lists.insert(lists.end(), places.begin() + first, places.end());
         int* staged = static_cast<int*>(rt.ws.raw("keep_lists", (4 + static_cast<size_t>(cache.max_context)) * sizeof(int)));
