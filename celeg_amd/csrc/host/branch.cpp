@@ -9,6 +9,9 @@
 namespace celeg {
 
 namespace {
+// A launch has fewer than 2^32 threads: more rows, pairs or requests than this are launched in turns.
+constexpr long long MOST_A_LAUNCH = 1 << 20;
+
 void need(bool ok, const char* message) {
     if (!ok) throw ArgumentError(message);
 }
@@ -59,18 +62,33 @@ static void check(const TokenLogprobs& a) {
     aligned({a.tokens, a.logprobs, a.ranks, a.entropy, a.top_ids, a.top_logprobs}, 4, "token_logprobs: lists and results must lie on boundaries of 4 bytes");
 }
 
+// rows of a launch: a workgroup or more for each
+static long long rows_at_once(const TokenLogprobs& a) { return std::min(a.rows, std::max(1LL, 8 * MOST_A_LAUNCH / (a.vocab / 1024 + 2))); }
+
 size_t token_logprobs_workspace(const TokenLogprobs& a) {
     check_sizes(a);
-    return a.rows ? celeg_logprobs_workspace(static_cast<int>(a.dtype), a.rows, static_cast<int>(a.vocab), a.per_row, a.top) : 0;
+    if (a.rows == 0) return 0;
+    // (the last launch's rows may be few, which are cut into more parts)
+    const long long most = rows_at_once(a), last = a.rows % most;
+    const auto bytes = [&](long long rows) {
+        return rows ? celeg_logprobs_workspace(static_cast<int>(a.dtype), rows, static_cast<int>(a.vocab), a.per_row, a.top) : 0;
+    };
+    return std::max(bytes(most), bytes(last));
 }
 
 void token_logprobs(const TokenLogprobs& a, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     check(a);
     if (a.rows == 0) return;
     check_workspace(workspace, workspace_bytes, token_logprobs_workspace(a));
-    kernel_check(celeg_logprobs_rows(a.logits, static_cast<int>(a.dtype), a.rows, static_cast<int>(a.vocab), a.row_stride, a.tokens,
-                                     a.per_row, a.top, a.logprobs, a.ranks, a.entropy, a.top_ids, a.top_logprobs, workspace, stream),
-                 "token_logprobs");
+    const long long most = rows_at_once(a);
+    const auto at = [](auto* list, long long offset) { return list ? list + offset : nullptr; };
+    for (long long first = 0; first < a.rows; first += most) {
+        const char* logits = static_cast<const char*>(a.logits) + first * a.row_stride * static_cast<long long>(dtype_size(a.dtype));
+        kernel_check(celeg_logprobs_rows(logits, static_cast<int>(a.dtype), std::min(most, a.rows - first), static_cast<int>(a.vocab), a.row_stride,
+                                         at(a.tokens, first * a.per_row), a.per_row, a.top, at(a.logprobs, first * a.per_row),
+                                         at(a.ranks, first * a.per_row), at(a.entropy, first), at(a.top_ids, first * a.top),
+                                         at(a.top_logprobs, first * a.top), workspace, stream), "token_logprobs");
+    }
 }
 
 // ---------------------------------------------------------------------------- attention of trees
@@ -82,7 +100,7 @@ static void check_sizes(const TreeAttention& a, const KVView& kv) {
     need(a.rows >= 0 && a.requests >= 0, "tree_attention: negative counts");
     need(a.heads > 0 && a.heads <= 65535 && a.heads % kv.kv_heads == 0, "tree_attention: heads must be a multiple of the cache's key/value heads");
     need(a.max_nodes > 0 && a.max_nodes <= TreeAttention::MAX_NODES, "tree_attention: max_nodes must be in [1, 256]");
-    need(static_cast<long long>(a.requests) * a.max_nodes <= 65535, "tree_attention: more than 65,535 requests times max_nodes");
+    need(static_cast<long long>(a.requests) * a.max_nodes <= TreeAttention::MAX_REQUEST_NODES, "tree_attention: more than 65,535 requests times max_nodes");
     need(a.window >= 0 && a.max_context >= 0, "tree_attention: window and max_context must not be negative");
     need(std::isfinite(a.scale), "tree_attention: the scale must be finite");
     const long long width = static_cast<long long>(a.heads) * kv.head_dim;
@@ -143,9 +161,11 @@ void move_tokens(const MoveTokens& a, const KVView& kv, hipStream_t stream) {
     if (a.requests == 0 || a.n_places == 0) return;
     need(a.src_slots && a.dst_slots && a.offsets && a.places && a.dst_starts, "move_tokens: an argument is missing");
     aligned({a.src_slots, a.dst_slots, a.offsets, a.places, a.dst_starts}, 4, "move_tokens: lists must lie on boundaries of 4 bytes");
-    kernel_check(celeg_move_token_list(kv.k, kv.v, static_cast<int>(kv.dtype), kv.n_pages, kv.n_layers, kv.kv_heads, kv.page_tokens,
-                                       kv.head_dim, kv.v_head_dim, kv.table, kv.table_rows, kv.table_stride, a.src_slots, a.dst_slots,
-                                       a.offsets, a.places, a.dst_starts, a.requests, a.n_places, stream), "move_tokens");
+    for (long long first = 0; first < a.requests; first += MOST_A_LAUNCH)
+        kernel_check(celeg_move_token_list(kv.k, kv.v, static_cast<int>(kv.dtype), kv.n_pages, kv.n_layers, kv.kv_heads, kv.page_tokens,
+                                           kv.head_dim, kv.v_head_dim, kv.table, kv.table_rows, kv.table_stride, a.src_slots + first,
+                                           a.dst_slots + first, a.offsets + first, a.places, a.dst_starts + first,
+                                           static_cast<int>(std::min(MOST_A_LAUNCH, a.requests - first)), a.n_places, stream), "move_tokens");
 }
 
 void copy_pages(const KVView& kv, const int* src, const int* dst, int n, hipStream_t stream) {
@@ -155,8 +175,9 @@ void copy_pages(const KVView& kv, const int* src, const int* dst, int n, hipStre
     need(src && dst, "copy_pages: the lists of pages are missing");
     aligned({src, dst}, 4, "copy_pages: lists must lie on boundaries of 4 bytes");
     const size_t per_dim = static_cast<size_t>(kv.n_layers) * kv.kv_heads * kv.page_tokens * dtype_size(kv.dtype);
-    kernel_check(celeg_copy_page_list(kv.k, kv.v, per_dim * kv.head_dim, per_dim * kv.v_head_dim, kv.n_pages, src, dst, n, stream),
-                 "copy_pages");
+    for (long long first = 0; first < n; first += MOST_A_LAUNCH)
+        kernel_check(celeg_copy_page_list(kv.k, kv.v, per_dim * kv.head_dim, per_dim * kv.v_head_dim, kv.n_pages, src + first, dst + first,
+                                          static_cast<int>(std::min(MOST_A_LAUNCH, n - first)), stream), "copy_pages");
 }
 
 }  // namespace celeg

@@ -43,6 +43,7 @@ struct TreeAttention {
     int max_nodes = 0;                     // most nodes of a request; what lies behind them is left alone
     int max_context = 0;                   // about the longest context (0: what the table holds); decides how the work is cut, nothing else
     static constexpr int MAX_NODES = 256, MAX_HEAD_DIM = 256;
+    static constexpr int MAX_REQUEST_NODES = 65535;      // requests times max_nodes of a call
 };
 size_t tree_attention_workspace(const TreeAttention& a, const KVView& kv);
 void tree_attention(const TreeAttention& a, const KVView& kv, void* workspace, size_t workspace_bytes, hipStream_t stream);

@@ -873,7 +873,7 @@ extern "C" int celeg_tree_attention_fast_ok(int head_dim, int page_tokens) {
     return (head_dim == 32 || head_dim == 64 || head_dim == 96 || head_dim == 128) && page_tokens >= 16 && (page_tokens & (page_tokens - 1)) == 0;
 }
 
-// Parts that the contexts are cut into.
+// Parts that the contexts are cut into (0: more workgroups than a launch has).
 //   Few rounds are one workgroup's: up to 12 (4 where keys are staged) a second kernel costs more than the wait (1 request of 8 nodes,
 // 16 heads of 64 on 8, behind 700: 9.2 us, in 3 parts 9.8, and a launch less for the host; behind 1,500: 13.3 and 10.6).
 //   More: 256 workgroups, one a compute unit, each wavefront (each workgroup that stages: two) with a round at least: a second one beside it
@@ -885,10 +885,16 @@ extern "C" int celeg_tree_attention_parts(int dtype, int head_dim, int requests,
     const TreeForm form = tree_form(dtype, head_dim, rows);
     const long long groups = static_cast<long long>(requests) * kv_heads * ((rows + form.rows - 1) / form.rows);
     const long long rounds = (static_cast<long long>(max_context) + max_nodes + form.keys - 1) / form.keys;
-    if (rounds <= (form.staged ? 4 : 12)) return 1;
+    // (a launch has fewer than 2^32 threads, here of up to 512 a workgroup)
+    const auto fits = [&](long long parts) {
+        return (groups * parts + 8LL * ((rows + form.rows - 1) / form.rows)) * 512 < 1LL << 32 &&
+               (parts == 1 || static_cast<long long>(requests) * max_nodes * kv_heads * group / 4 + 1 < 1LL << 24);
+    };
+    if (rounds <= (form.staged ? 4 : 12)) return fits(1) ? 1 : 0;
     long long parts = (256 + groups - 1) / groups;
     if (form.staged && form.resident > 1 && rounds > (head_dim > 64 ? 40 : 16) * parts) parts = (256 * form.resident + groups - 1) / groups;
-    return static_cast<int>(std::max(1LL, std::min({parts, form.staged ? (rounds + 1) / 2 : (rounds + 3) / 4, 64LL})));
+    parts = std::max(1LL, std::min({parts, form.staged ? (rounds + 1) / 2 : (rounds + 3) / 4, 64LL}));
+    return fits(parts) ? static_cast<int>(parts) : 0;
 }
 
 extern "C" int celeg_tree_attention_fast(const void* q, int ldq, int dtype, const void* k_pool, const void* v_pool, int n_pages, int n_layers,

@@ -155,12 +155,41 @@ static void failing_copies(const char* folder) {
     }
 }
 
+// lists of any length are launched (the stand-in ends the program at a launch that no GPU takes); kernels do not run, so nothing is read
+static void long_lists() {
+    void* const memory = reinterpret_cast<void*>(size_t(1) << 40);
+    int32_t* const list = static_cast<int32_t*>(memory);
+    celeg_paged_cache cache{sizeof(celeg_paged_cache), memory, memory, list, 1, 100, 2, 256, 16, 32, 32, 1, 8};
+    EXPECT(celeg_copy_pages(&cache, list, list, 2147483647, nullptr) == CELEG_OK);
+    EXPECT(celeg_move_tokens(&cache, 2147483646, list, list, list, list, 2147483647, list, nullptr) == CELEG_OK);
+    for (int64_t vocab : {1, 1500, 8193, 100003, 1 << 24})
+        for (int64_t rows : {1ll << 20, 1ll << 24, (1ll << 31) - 1}) {
+            celeg_token_logprobs_args a{sizeof(celeg_token_logprobs_args), memory, rows, vocab, vocab, 0, 1, 1, list, static_cast<float*>(memory), list,
+                                        static_cast<float*>(memory), list, static_cast<float*>(memory)};
+            size_t bytes = 0;
+            if (celeg_token_logprobs_workspace(&a, &bytes) != CELEG_OK) continue;      // (too many logits for a call)
+            EXPECT(celeg_token_logprobs(&a, memory, bytes, nullptr) == CELEG_OK);
+        }
+    for (int32_t kv_heads : {1, 8, 256, 60000}) {
+        cache.kv_heads = kv_heads;
+        cache.n_layers = 1;
+        for (int32_t nodes : {1, 40, 256}) {
+            celeg_tree_attention_args a{sizeof(celeg_tree_attention_args), memory, kv_heads * 32ll, memory, 9, kv_heads, 65535 / nodes, 0, list, list, list,
+                                        list, 1.f, 0, nodes, 100};
+            size_t bytes = 0;
+            EXPECT(celeg_tree_attention_workspace(&a, &cache, &bytes) == CELEG_OK);
+            EXPECT(celeg_tree_attention(&a, &cache, memory, bytes, nullptr) == CELEG_OK);
+        }
+    }
+}
+
 int main(int argc, char** argv) {
     if (argc != 3) return 2;
     requests(argv[1], true, 0, "float32");
     const size_t memory = hip_stand_in_memory();
     for (unsigned i = 1; i <= 12; ++i) requests(argv[1 + i % 2], i % 2 == 0, i, i % 4 < 2 ? "float32" : "bfloat16");
     failing_copies(argv[1]);
+    long_lists();
     EXPECT(hip_stand_in_memory() == memory);             // closed models leave nothing
     EXPECT(hip_stand_in_launches() > 1000);
     std::printf("failures: %d\n", failures);
