@@ -491,8 +491,8 @@ Tensor ModelRunner::step_of_trees(const std::vector<StepEntry>& entries) {
             if (e.parents[i] < -1 || e.parents[i] >= static_cast<int>(i))
                 throw StepError("step: parent " + std::to_string(e.parents[i]) + " of token " + std::to_string(i) + " is not before it");
     }
-    if (most > static_cast<size_t>(TreeAttention::MAX_NODES) || most * entries.size() > 65535)
-        throw StepError("step: trees of up to " + std::to_string(TreeAttention::MAX_NODES) + " tokens, up to 65,535 entries times the largest");
+    if (most > static_cast<size_t>(TreeAttention::MAX_NODES))
+        throw StepError("step: trees of up to " + std::to_string(TreeAttention::MAX_NODES) + " tokens");
     auto updates = drain_updates(std::vector<int>(static_cast<size_t>(cache.n_groups()), update_room_));
     BuildOptions options;
     options.null_slot = cache.null_slot;

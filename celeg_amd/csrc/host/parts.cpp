@@ -502,21 +502,24 @@ private:
             a.out = attended.data;
             a.rows = batch.n_tokens;
             a.heads = heads_;
-            a.requests = batch.n_seqs;
-            a.slots = batch.seq_slot;
-            a.starts = batch.seq_start;
-            a.offsets = batch.cu_seqlens;
             a.parents = batch.tree_parents;
             a.scale = scale_;
             a.window = window_ ? *window_ : 0;
             a.max_nodes = batch.max_tree_nodes;
             a.max_context = batch.context_hint();
-            // (room by powers of two: a workspace that grows with every longer context would keep all its former selves)
-            const size_t needed = tree_attention_workspace(a, *cache.kv);
-            size_t bytes = needed ? size_t(1) << 16 : 0;
-            while (bytes < needed) bytes *= 2;
             rt.ops.took(Path::AttentionTrees);
-            tree_attention(a, *cache.kv, bytes ? rt.ws.raw("tree_parts", bytes) : nullptr, bytes, rt.stream);
+            const int at_once = TreeAttention::MAX_REQUEST_NODES / a.max_nodes;
+            for (int first = 0; first < batch.n_seqs; first += at_once) {
+                a.requests = std::min(at_once, batch.n_seqs - first);
+                a.slots = batch.seq_slot + first;
+                a.starts = batch.seq_start + first;
+                a.offsets = batch.cu_seqlens + first;
+                // (room by powers of two: a workspace that grows with every longer context would keep all its former selves)
+                const size_t needed = tree_attention_workspace(a, *cache.kv);
+                size_t bytes = needed ? size_t(1) << 16 : 0;
+                while (bytes < needed) bytes *= 2;
+                tree_attention(a, *cache.kv, bytes ? rt.ws.raw("tree_parts", bytes) : nullptr, bytes, rt.stream);
+            }
             return attended;
         }
         // a decode-only step: the attention kernel prepares and writes the step's own keys and values

@@ -291,7 +291,7 @@ celeg_status celeg_token_logprobs_workspace(const celeg_token_logprobs_args* arg
 celeg_status celeg_token_logprobs(const celeg_token_logprobs_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Attention of drafted trees.  Request r has rows offsets[r] .. offsets[r + 1] - 1 of q and out (up to max_nodes, at most
- * 256): the nodes of its tree, whose keys and values lie behind its context of starts[r] tokens, node i's at place starts[r] + i
+ * 256; requests times max_nodes up to 65,535 a call): the nodes of its tree, whose keys and values lie behind its context of starts[r] tokens, node i's at place starts[r] + i
  * of slot slots[r].  parents[row] is the index inside the tree of the node's parent, lower than its own (anything else: a
  * root).  A node sees the context, its ancestors and itself, with a window only what stands fewer than `window` positions
  * before its own, starts[r] + depth.  out = softmax(scale q . k) v [rows, heads * head_dim], in the pages' dtype like q (rows

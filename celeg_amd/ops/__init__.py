@@ -137,8 +137,9 @@ def tree_attention(q: torch.Tensor, cache: PagedCache, layer: int, slots: torch.
     ``offsets[r]`` to ``offsets[r + 1] - 1``; their keys and values lie in ``cache`` behind the request's context, node i's at place
     ``starts[r] + i`` of slot ``slots[r]``.  ``parents[row]``: the parent's index inside the tree, -1 for a root.  A node sees the
     context, its ancestors and itself (with a ``window``: fewer than so many positions back).  ``scale`` defaults to
-    head_dim ** -0.5; ``max_nodes`` is the most nodes of a request (default: the rows, at most 256), ``max_context``
-    about the longest context (0: what the table holds), by which the work is cut.  ``out`` [rows, heads * head_dim] is
+    head_dim ** -0.5; ``max_nodes`` is the most nodes of a request (default: the rows, at most 256: of many requests it is worth saying,
+    as the work is cut by it; 1 where every request brings a single token), ``max_context`` about the longest context (0: what the
+    table holds), by which the work is cut.  ``out`` [rows, heads * head_dim] is
     made if it is not given; rows of no request are then undefined, and left as they were where it is."""
     if not isinstance(cache, PagedCache):
         _refuse("cache must be a PagedCache")
@@ -156,16 +157,22 @@ def tree_attention(q: torch.Tensor, cache: PagedCache, layer: int, slots: torch.
     elif not isinstance(out, torch.Tensor) or out.device != device or out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous():
         _refuse("out must be contiguous, of q's shape, dtype and device")
     requests = slots.shape[0] if isinstance(slots, torch.Tensor) and slots.dim() == 1 else -1
-    args = native.TreeAttentionArgs(
-        ctypes.sizeof(native.TreeAttentionArgs), q.data_ptr(), q_stride, out.data_ptr(), rows, width // cache.head_dim, requests, layer,
-        _ints(slots, "slots", requests, device), _ints(starts, "starts", requests, device), _ints(offsets, "offsets", requests + 1, device),
-        _ints(parents, "parents", rows, device), cache.head_dim ** -0.5 if scale is None else scale, window,
-        min(max(rows, 1), MAX_TREE_NODES) if max_nodes is None else max_nodes, max_context)
-    lib, ref, size = native.lib(), ctypes.byref(args), ctypes.c_size_t()
-    pages = cache._here()
-    native.check(lib.celeg_tree_attention_workspace(ref, pages, ctypes.byref(size)))
-    workspace = torch.empty(size.value, dtype=torch.uint8, device=device) if size.value else None
-    _call(device, lib.celeg_tree_attention, ref, pages, workspace.data_ptr() if size.value else None, size.value)
+    lists = (_ints(slots, "slots", requests, device), _ints(starts, "starts", requests, device), _ints(offsets, "offsets", requests + 1, device))
+    if max_nodes is None:
+        max_nodes = min(max(rows, 1), MAX_TREE_NODES)
+    # (a call of the library takes 65,535 requests times nodes: more requests go in several, each with its part of the lists)
+    most = max(1, 65535 // max_nodes) if max_nodes > 0 else requests
+    for first in range(0, requests, most) if requests > most else (0,):
+        n = min(requests - first, most)
+        args = native.TreeAttentionArgs(
+            ctypes.sizeof(native.TreeAttentionArgs), q.data_ptr(), q_stride, out.data_ptr(), rows, width // cache.head_dim, n, layer,
+            *(address + 4 * first for address in lists), _ints(parents, "parents", rows, device), cache.head_dim ** -0.5 if scale is None else scale,
+            window, max_nodes, max_context)
+        lib, ref, size = native.lib(), ctypes.byref(args), ctypes.c_size_t()
+        pages = cache._here()
+        native.check(lib.celeg_tree_attention_workspace(ref, pages, ctypes.byref(size)))
+        workspace = torch.empty(size.value, dtype=torch.uint8, device=device) if size.value else None
+        _call(device, lib.celeg_tree_attention, ref, pages, workspace.data_ptr() if size.value else None, size.value)
     return out
 
 

@@ -1,13 +1,28 @@
 """``celeg_amd.ops`` with more requests, rows and pairs than one launch or one call of the library takes."""
+import random
+
 import pytest
 import torch
 
 from celeg_amd import ops
 
 import plain_branch as plain
+from test_gpu_branch_ops import Trees
 
 pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("dim", [64, 40])
+def test_trees_of_many_requests_without_a_bound_on_their_nodes(dim, dtype):
+    """600 requests of which one has 200 nodes, most a few and some none: the rows alone do not say how many a request has."""
+    rng = random.Random(dim)
+    nodes = [rng.choice([0, 1, 1, 1, 2, 5]) for _ in range(600)]
+    nodes[417] = 200
+    t = Trees([rng.randint(0, 30) for _ in nodes], nodes, 4, 2, dim, dtype, layers=1, seed=dim)
+    t.check()
+    t.check(window=9)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
