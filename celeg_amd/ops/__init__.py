@@ -22,6 +22,7 @@ from ..native import NativeArgumentError
 MAX_TOKENS_PER_ROW = 8
 MAX_TOP = 128
 MAX_TREE_NODES = 256
+_MAX_REQUEST_NODES = 65535       # requests times nodes of a call of the library
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
@@ -130,6 +131,13 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     return TokenLogprobs(logprobs, ranks, entropy, top_ids, top_logprobs)
 
 
+def _attend(device: torch.device, args: native.TreeAttentionArgs, pages) -> None:
+    lib, ref, size = native.lib(), ctypes.byref(args), ctypes.c_size_t()
+    native.check(lib.celeg_tree_attention_workspace(ref, pages, ctypes.byref(size)))
+    workspace = torch.empty(size.value, dtype=torch.uint8, device=device) if size.value else None
+    _call(device, lib.celeg_tree_attention, ref, pages, workspace.data_ptr() if size.value else None, size.value)
+
+
 def tree_attention(q: torch.Tensor, cache: PagedCache, layer: int, slots: torch.Tensor, starts: torch.Tensor, offsets: torch.Tensor,
                    parents: torch.Tensor, *, scale: Optional[float] = None, window: int = 0, max_nodes: Optional[int] = None,
                    max_context: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -157,22 +165,22 @@ def tree_attention(q: torch.Tensor, cache: PagedCache, layer: int, slots: torch.
     elif not isinstance(out, torch.Tensor) or out.device != device or out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous():
         _refuse("out must be contiguous, of q's shape, dtype and device")
     requests = slots.shape[0] if isinstance(slots, torch.Tensor) and slots.dim() == 1 else -1
-    lists = (_ints(slots, "slots", requests, device), _ints(starts, "starts", requests, device), _ints(offsets, "offsets", requests + 1, device))
+    slots_at, starts_at = _ints(slots, "slots", requests, device), _ints(starts, "starts", requests, device)
+    offsets_at, parents_at = _ints(offsets, "offsets", requests + 1, device), _ints(parents, "parents", rows, device)
     if max_nodes is None:
         max_nodes = min(max(rows, 1), MAX_TREE_NODES)
-    # (a call of the library takes 65,535 requests times nodes: more requests go in several, each with its part of the lists)
-    most = max(1, 65535 // max_nodes) if max_nodes > 0 else requests
-    for first in range(0, requests, most) if requests > most else (0,):
-        n = min(requests - first, most)
-        args = native.TreeAttentionArgs(
-            ctypes.sizeof(native.TreeAttentionArgs), q.data_ptr(), q_stride, out.data_ptr(), rows, width // cache.head_dim, n, layer,
-            *(address + 4 * first for address in lists), _ints(parents, "parents", rows, device), cache.head_dim ** -0.5 if scale is None else scale,
-            window, max_nodes, max_context)
-        lib, ref, size = native.lib(), ctypes.byref(args), ctypes.c_size_t()
-        pages = cache._here()
-        native.check(lib.celeg_tree_attention_workspace(ref, pages, ctypes.byref(size)))
-        workspace = torch.empty(size.value, dtype=torch.uint8, device=device) if size.value else None
-        _call(device, lib.celeg_tree_attention, ref, pages, workspace.data_ptr() if size.value else None, size.value)
+    args = native.TreeAttentionArgs(
+        ctypes.sizeof(native.TreeAttentionArgs), q.data_ptr(), q_stride, out.data_ptr(), rows, width // cache.head_dim, requests, layer,
+        slots_at, starts_at, offsets_at, parents_at, cache.head_dim ** -0.5 if scale is None else scale, window, max_nodes, max_context)
+    if requests * max_nodes <= _MAX_REQUEST_NODES or max_nodes < 1:
+        _attend(device, args, cache._here())
+        return out
+    # more requests than a call of the library takes: several, each with its part of the lists
+    most = max(1, _MAX_REQUEST_NODES // max_nodes)
+    for first in range(0, requests, most):
+        args.requests = min(requests - first, most)
+        args.slots, args.starts, args.offsets = slots_at + 4 * first, starts_at + 4 * first, offsets_at + 4 * first
+        _attend(device, args, cache._here())
     return out
 
 
