@@ -114,7 +114,7 @@ __device__ __forceinline__ unsigned quotient(unsigned x, unsigned by, unsigned d
 // where a request moves a few tokens, so that the way to them (slots, places, table) is gone once.  A run has as many tokens as its
 // workgroup's threads hold, MOVE_EACH pieces (groups) a thread.
 // Bound by the bytes: 8 requests that keep 4,001 to 3,500 of 8,192 tokens, 6 layers of 8 heads of 64 in bfloat16 (737 MB, and the values
-// that lie between those kept, 184 MB): 219 us, 4.2 TB/s; the keys alone 82 us, 4.5 TB/s.  Sixteen tokens' groups side by side in
+// that lie between those kept, 184 MB): 212 us, 4.3 TB/s; the keys alone 82 us, 4.5 TB/s.  Sixteen tokens' groups side by side in
 // neighbouring lanes, so that a store writes whole lines: 277 -> 226 us.
 #define MOVE_EACH 4
 #define MOVE_RUN 256             // most tokens of a run

@@ -297,7 +297,8 @@ celeg_status celeg_token_logprobs(const celeg_token_logprobs_args* args, void* w
  * before its own, starts[r] + depth.  out = softmax(scale q . k) v [rows, heads * head_dim], in the pages' dtype like q (rows
  * q_stride elements apart).  Rows of no request, of a request behind max_nodes, or of a slot outside the table are left as
  * they were.  What a node does not see may hold anything, infinities and NaN included; a node that sees nothing (none of its
- * places has a page) gets zeros. */
+ * places has a page) gets zeros.  In bfloat16 the weights of the softmax are rounded to bfloat16 where the matrix cores take the sizes (heads of
+ * 32, 64, 96 or 128, pages of a power of two from 16 tokens on, addresses and rows on 16 bytes); elsewhere they keep 32 bits. */
 typedef struct celeg_tree_attention_args {
     size_t struct_size;
     const void* q;
@@ -315,8 +316,9 @@ celeg_status celeg_tree_attention(const celeg_tree_attention_args* args, const c
 
 /* Keys and values of all layers moved: entry i of request r (entries offsets[r] .. offsets[r + 1] - 1 of places) goes from place
  * places[entry] of slot src_slots[r] to place dst_starts[r] + i of slot dst_slots[r].  Within one slot the places have to rise,
- * none above where its token goes to (place >= dst_starts[r] + i); between two slots any order will do.  No place that one request writes
- * may be one that another reads or writes.  A place outside the table, or on no page, is left out. */
+ * none below where its token goes to (place >= dst_starts[r] + i); between two slots any order will do, if none of the tokens read lies
+ * where one is written (two slots that share a page: forked ones).  No place that one request writes may be one that another reads or
+ * writes.  A place outside the table, or on no page, is left out. */
 celeg_status celeg_move_tokens(const celeg_paged_cache* cache, int32_t requests, const int32_t* src_slots, const int32_t* dst_slots,
                                const int32_t* offsets, const int32_t* places, int32_t n_places, const int32_t* dst_starts, void* stream);
 

@@ -9,10 +9,10 @@
 // What bounds it is the one read of the logits.  A workgroup of 256 threads takes a part of a row into its registers (up to
 // 64 logits a thread), and finds there in turn the maximum, the sums, the tokens' ranks and the part's best: four such
 // workgroups share a compute unit, so that one's arithmetic runs while another's loads are on their way; a second kernel, a
-// workgroup a row, joins the parts.  2,048 rows of 65,536 32-bit logits, 5 best: 104 us (5.2 TB/s, as a large copy); of bfloat16 80 us,
+// workgroup a row, joins the parts.  2,048 rows of 65,536 32-bit logits, 5 best: 106 us (5.1 TB/s, as a large copy); of bfloat16 80 us,
 // bound by the vector instructions (an exponential is four of the about 20 a logit).  Up to 256 rows, one a compute unit, have
-// nothing to overlap with: there a workgroup of 1,024 threads takes a whole row of up to 65,536 logits, and nothing is joined (one row 11.0
-// us where parts and their join take 12.0, and a launch and a workspace less for the host; 64 rows, 20 best 12.1 and 14.7; 128 best
+// nothing to overlap with: there a workgroup of 1,024 threads takes a whole row of up to 65,536 logits, and nothing is joined (one row 10.6
+// us where parts and their join take 12.0, and a launch and a workspace less for the host; 64 rows, 20 best 12.5 and 14.7; 128 best
 // of one row 25 and 140).
 //
 // The best of a part: the top-th largest of the maxima of 64 (256) groups of threads is not above the top-th largest logit,
@@ -63,7 +63,7 @@ struct LogprobOut {
     float* top_logprobs;
 };
 
-// What a part of a row leaves for the join.  stats: m, S, T, and how its order stands (1: a NaN).
+// What a part of a row leaves for the join.  stats: m, S and T (against m log2(e) as rounded), and how its order stands (1: a NaN).
 struct LogprobParts {
     float4* stats;                   // [rows, parts]
     int* ranks;                      // [rows, parts, per_row]

@@ -10,9 +10,13 @@
 // for once for many rows.  Up to 32 rows: a workgroup's four wavefronts take rounds of keys in turn, each with a running maximum,
 // sum and output of its own, and meet in LDS.  More, in bfloat16: 64, 128 or 256 rows a workgroup share rounds of 64 keys that are
 // staged in LDS.  Long contexts are cut into parts for as many workgroups, which a second kernel joins.
-// Bound by: few rows, the bytes of keys and values (16 trees of 16 nodes behind 12,001 to 16,384 tokens, 32 heads of 128 on 8: 204
-// us, 5.2 TB/s) or, in short contexts, a chain of reads; many rows, vector and matrix instructions (of 64 nodes: 326 us, 730 TFLOP/s,
-// 2.9 TB/s, of which 14 us join two parts).
+// Bound by: few rows, the bytes of keys and values (16 trees of 1 node behind 12,001 to 16,384 tokens, 32 heads of 128 on 8: 175
+// us, 5.3 TB/s, of 16 nodes 183) or, in short contexts, a chain of reads; many rows, vector and matrix instructions (of 64 nodes: 335 us, 710
+// TFLOP/s, 2.8 TB/s, of which 14 us join two parts).
+//
+// Scores, maxima, sums and outputs are 32-bit.  In bfloat16 the weights enter the product with the values rounded to bfloat16 (half a step each,
+// 2^-8; the sum is of the exact ones); the kernel for any sizes, which has no matrix instructions, keeps them in 32 bits.  Against 64 bits
+// results are off by 0.0022 of their size here, of which their own rounding is 0.0017.
 #include "common.h"
 #include <algorithm>
 #include <climits>
@@ -852,8 +856,8 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeArgs a) {
 // that a compute unit holds.
 //   Up to 32 rows nothing is gained by staging: four wavefronts read 16 or 32 rows' keys themselves.  Above, staged: 64 rows by four
 // wavefronts, 128 by four with two row tiles each, and more by eight, which read every key once for 256 rows, from four buffers (16
-// trees of 64 nodes behind 12,001 to 16,384 tokens, 32 heads of 128 on 8: 378 us, in workgroups of 128 rows 437; heads of 64 252 and
-// 278; 8 trees of 64 behind 8,192 tokens, heads of 64: 72 and 75).
+// trees of 64 nodes behind 16,384 tokens, 32 heads of 128 on 8: 368 us, in workgroups of 128 rows 419; behind 14,192, heads of 64: 205 and
+// 221; 8 trees of 64 behind 8,192 tokens, heads of 64: 69 and 72, of 128 112 and 119).
 struct TreeForm {
     bool staged;
     int tiles, rows, keys, resident;
@@ -875,11 +879,16 @@ extern "C" int celeg_tree_attention_fast_ok(int head_dim, int page_tokens) {
 
 // Parts that the contexts are cut into (0: more workgroups than a launch has).
 //   Few rounds are one workgroup's: up to 12 (4 where keys are staged) a second kernel costs more than the wait (1 request of 8 nodes,
-// 16 heads of 64 on 8, behind 700: 9.2 us, in 3 parts 9.8, and a launch less for the host; behind 1,500: 13.3 and 10.6).
+// 16 heads of 64 on 8, behind 500, 700, 760, 900, 1,100 and 1,500: 8.4, 9.3, 9.6, 10.5, 11.6 and 13.6 us, in the best number of parts 9.8,
+// 10.6, 10.8, 10.3, 10.4 and 10.4, and a launch less for the host; of 4 requests behind 760 and 1,100 11.8 and 13.8, 12.6 and 11.9).  In 32 bits, whose
+// rounds take longer, the two meet earlier (3 of 13 behind 200, 300 and 500: 12.9, 15.6 and 20.3, 13.2, 13.4 and 14.0), but a launch more
+// is the host's.
 //   More: 256 workgroups, one a compute unit, each wavefront (each workgroup that stages: two) with a round at least: a second one beside it
 // gains less than its part costs to join (4 trees of 8 behind 6,000, 32 heads of 64 on 8: 20.0 us, of 512 workgroups 22.9; heads
-// of 128 29.7 and 34.9; 4 of 26 behind 2,500, staged: 16.7 and 21.3).  Staged rounds in long parts, more than 16 of them (40 of wider
-// heads), gain more (8 of 26 behind 16,000: 74 us, of 256 workgroups 85, heads of 128 123 and 135; behind 2,500 26 and 26, 36 and 34).
+// of 128 29.7 and 34.9).  Staged rounds in long parts gain more from it; the limits, 16 rounds a part and 40 of wider heads, lie where no case loses.
+// Heads of 64, 8 trees of 26 behind 2,500, 4,000, 6,000 and 16,000 (10, 16, 24 and 63 rounds a part of 256 workgroups): 25.6, 30.2, 39.2 and 84
+// us, of 512 25.3, 27.3, 34.5 and 70; 4 trees (5, 8, 12 and 31) 18.5, 21.1, 26.2 and 46, 19.2, 21.7, 25.1 and 40.  Heads of 128, 8 trees behind 6,000, 8,000
+// and 16,000 (24, 31 and 63) 60, 77 and 134, 61, 73 and 121; 4 trees behind 8,000, 11,000 and 16,000 (16, 22 and 31) 40, 54 and 74, 47, 57 and 72.
 extern "C" int celeg_tree_attention_parts(int dtype, int head_dim, int requests, int kv_heads, int group, int max_nodes, int max_context) {
     const int rows = max_nodes * group;
     const TreeForm form = tree_form(dtype, head_dim, rows);

@@ -188,7 +188,8 @@ def move_tokens(cache: PagedCache, src_slots: torch.Tensor, dst_slots: torch.Ten
                 dst_starts: torch.Tensor) -> None:
     """Keys and values of all layers: for every request r, the tokens at places ``places[offsets[r]:offsets[r + 1]]`` of slot
     ``src_slots[r]`` go to the places ``dst_starts[r]``, ``dst_starts[r] + 1``, .. of slot ``dst_slots[r]``.  Within one slot the places
-    have to rise and no token may move up; no place that a request writes may be one that another reads or writes."""
+    have to rise and no token may move up; between two, none that is read may lie where one is written (forked slots share pages). No place
+    that a request writes may be one that another reads or writes."""
     if not isinstance(cache, PagedCache):
         _refuse("cache must be a PagedCache")
     device = cache.device
