@@ -221,6 +221,7 @@ std::vector<int> CacheManager::pages_needed(int slot, int start_pos, int n_new) 
 
 std::vector<int> CacheManager::shared_pages(const Group& g, int slot, int start_pos, int n) const {
     std::vector<int> out;
+    if (n <= 0) return out;
     const auto& pages = g.pages[static_cast<size_t>(slot)];
     const int end = std::min((start_pos + n - 1) / page_tokens + 1, static_cast<int>(pages.size()));
     for (int idx = std::max(start_pos, 0) / page_tokens; idx < end; ++idx)
