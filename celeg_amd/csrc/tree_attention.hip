@@ -11,8 +11,8 @@
 // sum and output of its own, and meet in LDS.  More, in bfloat16: 64, 128 or 256 rows a workgroup share rounds of 64 keys that are
 // staged in LDS.  Long contexts are cut into parts for as many workgroups, which a second kernel joins.
 // Bound by: few rows, the bytes of keys and values (16 trees of 1 node behind 12,001 to 16,384 tokens, 32 heads of 128 on 8: 175
-// us, 5.3 TB/s, of 16 nodes 183) or, in short contexts, a chain of reads; many rows, vector and matrix instructions (of 64 nodes: 335 us, 710
-// TFLOP/s, 2.8 TB/s, of which 14 us join two parts).
+// us, 5.3 TB/s, of 16 nodes 183) or, in short contexts, a chain of reads; many rows, vector and matrix instructions (of 64 nodes: 319 to 335
+// us, by the clock, 710 to 745 TFLOP/s, 2.8 to 2.9 TB/s; 14 us of it join two parts).
 //
 // Scores, maxima, sums and outputs are 32-bit.  In bfloat16 the weights enter the product with the values rounded to bfloat16 (half a step each,
 // 2^-8; the sum is of the exact ones); the kernel for any sizes, which has no matrix instructions, keeps them in 32 bits.  Against 64 bits
